@@ -257,6 +257,52 @@ int pir_mlp_backward_tangent(const void* packed, size_t mats_floats, const PirMl
                              long P, const float* g_out, const float* gbar_x, float* ghat_out, float* const* gw,
                              void* scratch, size_t scratch_bytes, void* stream);
 
+/* ---- optimizer: AdamW over many tensors in one call (render_surface.py:213-231 builds one torch.optim.Adam per
+ *      network; with weight_decay = 0 this is the same step) -------------------------------------------------------- */
+
+/* Types of parameters and gradients. */
+enum { PIR_F32 = 0, PIR_BF16 = 1, PIR_F16 = 2 };
+
+/* Hyper-parameters shared by some of the tensors.  lr_device: optional DEVICE float that replaces lr (a captured graph
+ * reads it at every replay). */
+typedef struct PirAdamwGroup {
+  double lr, beta1, beta2, eps, weight_decay;
+  const float* lr_device;
+} PirAdamwGroup;
+
+/* Workspace of pir_adamw_step; with_norm: max_norm > 0, skip_nonfinite or total_norm is asked for. */
+size_t pir_adamw_workspace_bytes(int n, const long* numels, int with_norm);
+
+/* One step of n tensors.  Every array is a HOST array of n entries; params, grads, exp_avgs, exp_avg_sqs, scales and
+ * steps hold DEVICE pointers.  With t = *steps[i] + 1 and g the gradient (times min(1, max_norm / (|g| + 1e-6)), |g| the
+ * joint 2-norm of all n gradients, if max_norm > 0):
+ *   m = beta1 m + (1 - beta1) g,  v = beta2 v + (1 - beta2) g^2,
+ *   p = p - lr weight_decay p - lr / (1 - beta1^t) m / (sqrt(v / (1 - beta2^t)) + eps),  *steps[i] = t.
+ * params[i] and grads[i]: numels[i] values of type dtypes[i].  scales NULL or scales[i] NULL: exp_avgs[i] and
+ * exp_avg_sqs[i] are fp32[numels[i]].  Otherwise they are 8-bit codes, int8 and uint8 [ceil(numels[i] / 256) * 256],
+ * and scales[i] is fp32 [ceil(numels[i] / 256)][2]: m = s0 (q / 127) |q / 127|, v = s1 (c / 255)^4, s0 and s1 the
+ * largest |m| and v of 256 consecutive elements (codes aligned to 16 bytes, scales to 8; what lies behind numels[i] is written as zero).  A
+ * moment that is not finite makes its block's scale NaN.  groups[i]: index into group.  skip_nonfinite: if |g| is not
+ * finite nothing changes, the step counts included.  total_norm: optional DEVICE float that receives |g|.
+ * No two tensors of a call may overlap. */
+int pir_adamw_step(int n, void* const* params, const void* const* grads, void* const* exp_avgs, void* const* exp_avg_sqs,
+                   float* const* scales, float* const* steps, const long* numels, const int* dtypes, const int* groups,
+                   const PirAdamwGroup* group, int n_groups, double max_norm, int skip_nonfinite, float* total_norm,
+                   void* workspace, size_t workspace_bytes, void* stream);
+
+/* 2-norms of n tensors: *total (DEVICE) of all of them together, each[n] (DEVICE, or NULL) of every one.  Squares and
+ * sums in 64 bits, in a fixed order.  grads, numels, dtypes: HOST arrays as above. */
+size_t pir_grad_norm_workspace_bytes(int n, const long* numels);
+int pir_grad_norm(int n, const void* const* grads, const long* numels, const int* dtypes, float* total, float* each,
+                  void* workspace, size_t workspace_bytes, void* stream);
+
+/* 8-bit moments -> values of type dtype, [n_blocks][256] each. */
+int pir_moments8_decode(long n_blocks, const signed char* exp_avg, const unsigned char* exp_avg_sq, const float* scales,
+                        int dtype, void* m, void* v, void* stream);
+/* numel values of type dtype -> 8-bit moments of ceil(numel / 256) blocks, the last one filled up with zeros. */
+int pir_moments8_encode(long numel, int dtype, const void* m, const void* v, signed char* exp_avg,
+                        unsigned char* exp_avg_sq, float* scales, void* stream);
+
 /* ---- measurement aid (no counterpart in the reference) ------------------------------------------------ */
 
 /* Kernel families timed by the optional HIP-event profiler. */

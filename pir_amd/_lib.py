@@ -96,6 +96,18 @@ def _declare(L):
     L.pir_mlp_backward.argtypes = [vp, sz, vp, i32, vp, lg, vp, vp, ctypes.POINTER(vp), ctypes.POINTER(vp), vp, sz, vp]
     L.pir_mlp_backward_tangent.restype = i32
     L.pir_mlp_backward_tangent.argtypes = [vp, sz, vp, i32, vp, lg, vp, vp, vp, ctypes.POINTER(vp), vp, sz, vp]
+    L.pir_adamw_workspace_bytes.restype = sz
+    L.pir_adamw_workspace_bytes.argtypes = [i32, vp, i32]
+    L.pir_adamw_step.restype = i32
+    L.pir_adamw_step.argtypes = [i32] + [vp] * 10 + [i32, ctypes.c_double, i32, vp, vp, sz, vp]
+    L.pir_grad_norm_workspace_bytes.restype = sz
+    L.pir_grad_norm_workspace_bytes.argtypes = [i32, vp]
+    L.pir_grad_norm.restype = i32
+    L.pir_grad_norm.argtypes = [i32] + [vp] * 6 + [sz, vp]
+    L.pir_moments8_decode.restype = i32
+    L.pir_moments8_decode.argtypes = [lg, vp, vp, vp, i32, vp, vp, vp]
+    L.pir_moments8_encode.restype = i32
+    L.pir_moments8_encode.argtypes = [lg, i32, vp, vp, vp, vp, vp, vp]
     L.pir_profile_enable.restype = i32
     L.pir_profile_enable.argtypes = [i32]
     L.pir_profile_read.restype = i32

@@ -1,0 +1,485 @@
+"""AdamW over many tensors in one call, with both moments in 32 or in 8 bits, and gradient norms (pir_adamw_step,
+pir_grad_norm and pir_moments8_* in include/pir_hip.h; reference: one torch.optim.Adam per network,
+render_surface.py:213-231).
+
+  AdamW             a torch.optim.Optimizer; weight_decay=0 is torch.optim.Adam's step
+  step_together     one step of several AdamW optimizers in one call, with one joint gradient norm
+  adamw_step        the step itself on lists of tensors, moments in fp32
+  adamw8_step       the same with the moments in 8 bits and a scale per 256 elements
+  moments8_encode   fp32 / bf16 / fp16 moments -> 8-bit ones, and back: moments8_decode
+  grad_norm         the 2-norm of every tensor and of all together
+
+With t the step count of a tensor and g its gradient, times min(1, max_norm / (|g| + 1e-6)) where max_norm is given:
+
+  m = beta1 m + (1 - beta1) g        v = beta2 v + (1 - beta2) g^2
+  p = p (1 - lr weight_decay) - lr / (1 - beta1^t) m / (sqrt(v / (1 - beta2^t)) + eps)
+
+computed in fp32 and rounded once to p's type (fp32, bf16 or fp16; gradients have the type of their parameter).  The 8-bit
+moments of 256 consecutive elements are m = a (q / 127) |q / 127| (int8 q) and v = b (c / 255)^4 (uint8 c) with a, b the
+block's largest |m| and v in fp32, rounded to the nearest code, except that a v above zero keeps c >= 1.  A block whose
+largest is below 2^-126 is zero; one that holds an infinity or a NaN has a scale of NaN, as that element would have
+moments of NaN in 32 bits: skip_nonfinite leaves everything as it is in such a step.
+
+Step counts live on the device (fp32, one per tensor), so that a step can be captured into a HIP graph and replayed; a
+learning rate that changes between replays is a one-element fp32 device tensor.  Calls enqueue work on the current stream
+of the tensors' device and return without waiting.  Tensors on the CPU take the same formulas in torch operations.
+"""
+import ctypes
+import math
+from array import array
+
+import torch
+
+from . import _lib
+
+BLOCK = 256                      # elements that share a scale
+_TINY = 2.0 ** -126              # blocks whose largest is below this are zero
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+class _Group(ctypes.Structure):
+    _fields_ = [(k, ctypes.c_double) for k in ("lr", "beta1", "beta2", "eps", "weight_decay")] + [("lr_device", ctypes.c_void_p)]
+
+
+def _hyper(lr, betas, eps, weight_decay, device):
+    """Checked hyper-parameters of one group; a learning rate on the device stays there."""
+    dev_lr = None
+    if isinstance(lr, torch.Tensor):
+        if lr.numel() != 1:
+            raise ValueError("lr: a number or a tensor of one element")
+        if lr.is_cuda:
+            if lr.dtype != torch.float32 or lr.device != device:
+                raise ValueError("lr: a device tensor has to be float32, on the device of the parameters")
+            dev_lr, lr = lr, 0.0
+    lr, beta1, beta2 = float(lr), float(betas[0]), float(betas[1])
+    if not 0.0 <= lr < math.inf:
+        raise ValueError(f"lr out of range: {lr}")
+    if not (0.0 <= beta1 < 1.0 and 0.0 <= beta2 < 1.0):
+        raise ValueError(f"betas out of range: {betas}")
+    if not (0.0 <= float(eps) < math.inf and 0.0 <= float(weight_decay) < math.inf):
+        raise ValueError(f"eps or weight_decay out of range: {eps}, {weight_decay}")
+    return dev_lr, lr, beta1, beta2, float(eps), float(weight_decay)
+
+
+def _max_norm(max_norm):
+    """The bound of the joint norm for the kernels: 0 = no clipping."""
+    if max_norm is None:
+        return 0.0
+    max_norm = float(max_norm)
+    if not max_norm > 0.0:
+        raise ValueError(f"max_norm has to be positive: {max_norm}")
+    return max_norm if max_norm < math.inf else 0.0
+
+
+def _dense(t):
+    """Whether t's elements fill one stretch of memory, each once, in some order of its dimensions."""
+    if t.is_contiguous():
+        return True
+    want = 1
+    for size, stride in sorted(((s, d) for s, d in zip(t.shape, t.stride()) if s != 1), key=lambda x: x[1]):
+        if stride != want:
+            return False
+        want *= size
+    return True
+
+
+def _blocks(numel):
+    return -(-numel // BLOCK)
+
+
+def _check_disjoint(what, tensors):
+    """Kernels write these tensors side by side: no byte may belong to two of them."""
+    at = [(t.data_ptr(), t.numel() * t.element_size()) for t in tensors]
+    end = 0
+    for start, size in at:
+        if start < end:
+            break
+        end = start + size
+    else:
+        return
+    end = 0
+    for start, size in sorted(x for x in at if x[1]):
+        if start < end:
+            raise ValueError(f"{what}: a tensor is given twice, or two of them overlap")
+        end = start + size
+
+
+def _same_layout(p, t):
+    return t.shape == p.shape and (t.stride() == p.stride() or (t.is_contiguous() and p.is_contiguous()))
+
+
+def _check(params, grads, exp_avgs, exp_avg_sqs, scales):
+    """Checks the lists of one device; gradients that are laid out unlike their parameters come back as copies."""
+    n = len(params)
+    if not len(grads) == len(exp_avgs) == len(exp_avg_sqs) == n or (scales is not None and len(scales) != n):
+        raise ValueError("params, grads and moments: lists of one length")
+    dev = params[0].device
+    out = []
+    for i, (p, g, m, v) in enumerate(zip(params, grads, exp_avgs, exp_avg_sqs)):
+        if p.dtype not in _DTYPES:
+            raise ValueError(f"parameter {i}: {p.dtype} is not supported (float32, bfloat16, float16)")
+        if g is None or g.layout is not torch.strided or g.dtype != p.dtype or g.shape != p.shape:
+            raise ValueError(f"gradient {i}: a dense tensor of its parameter's shape and type is wanted")
+        if not (p.device == dev and g.device == dev and m.device == dev and v.device == dev):
+            raise ValueError(f"tensors {i}: on another device than parameter 0")
+        if not p.is_contiguous() and not _dense(p):
+            raise ValueError(f"parameter {i}: its elements do not fill one stretch of memory (strides {p.stride()})")
+        s = scales[i] if scales is not None else None
+        if s is None:
+            if m.dtype != torch.float32 or v.dtype != torch.float32 or not (_same_layout(p, m) and _same_layout(p, v)):
+                raise ValueError(f"moments {i}: float32 with their parameter's shape and strides are wanted")
+        else:
+            nb = _blocks(p.numel())
+            if m.dtype != torch.int8 or v.dtype != torch.uint8 or s.dtype != torch.float32 or s.device != dev \
+                    or tuple(m.shape) != (nb, BLOCK) or tuple(v.shape) != (nb, BLOCK) or tuple(s.shape) != (nb, 2) \
+                    or not (m.is_contiguous() and v.is_contiguous() and s.is_contiguous()):
+                raise ValueError(f"moments {i}: contiguous int8 and uint8 [{nb}, {BLOCK}] with float32 scales [{nb}, 2] are wanted")
+            if (m.data_ptr() | v.data_ptr()) % 16 or s.data_ptr() % 8:
+                raise ValueError(f"moments {i}: codes have to start at a multiple of 16 bytes, scales of 8")
+        if g.is_neg() or not _same_layout(p, g):
+            g = torch.empty_like(p, requires_grad=False).copy_(g)
+        out.append(g)
+    _check_disjoint("params", params)
+    _check_disjoint("first moments", exp_avgs)
+    _check_disjoint("second moments", exp_avg_sqs)
+    return out
+
+
+def _addresses(tensors):
+    return array("Q", [0 if t is None else t.data_ptr() for t in tensors])
+
+
+def _at(a):
+    return a.buffer_info()[0]
+
+
+def _on(device):
+    return torch.cuda.device(device)
+
+
+def _written(tensors):
+    """The kernels write through pointers: autograd and the packed copies of the networks' weights go by the version."""
+    live = [t for t in tensors if not t.is_inference()]
+    if live:
+        torch.autograd.graph.increment_version(live)
+
+
+def _run(params, grads, exp_avgs, exp_avg_sqs, scales, steps, groups, hypers, max_norm, skip_nonfinite, want_norm):
+    """One pir_adamw_step.  steps: addresses of the step counts; groups: index into hypers of each tensor."""
+    dev = params[0].device
+    n = len(params)
+    numels = array("q", [p.numel() for p in params])
+    dtypes = array("i", [_DTYPES[p.dtype] for p in params])
+    table = (_Group * len(hypers))()
+    for row, (dev_lr, lr, beta1, beta2, eps, decay) in zip(table, hypers):
+        row.lr, row.beta1, row.beta2, row.eps, row.weight_decay = lr, beta1, beta2, eps, decay
+        row.lr_device = None if dev_lr is None else dev_lr.data_ptr()
+    with_norm = want_norm or skip_nonfinite or max_norm > 0.0
+    L = _lib.lib()
+    arrays = [_addresses(x) for x in (params, grads, exp_avgs, exp_avg_sqs)]
+    arrays.append(_addresses(scales) if scales is not None else None)
+    with _on(dev):
+        norm = torch.empty((), dtype=torch.float32, device=dev) if with_norm else None
+        size = L.pir_adamw_workspace_bytes(n, _at(numels), int(with_norm))
+        work = torch.empty(size, dtype=torch.uint8, device=dev)
+        _lib.check(L.pir_adamw_step(n, *[None if a is None else _at(a) for a in arrays], _at(steps), _at(numels), _at(dtypes),
+                                    _at(groups), ctypes.addressof(table), len(hypers), max_norm, int(skip_nonfinite),
+                                    None if norm is None else norm.data_ptr(), work.data_ptr(), size,
+                                    torch.cuda.current_stream(dev).cuda_stream), "pir_adamw_step")
+    _written(params)
+    return norm
+
+
+def _run_torch(params, grads, exp_avgs, exp_avg_sqs, scales, steps, groups, hypers, max_norm, skip_nonfinite, want_norm):
+    """The same step in torch operations, for tensors on the CPU.  steps: the step counts, one-element tensors."""
+    with torch.no_grad():
+        norm, factor = None, 1.0
+        if want_norm or skip_nonfinite or max_norm > 0.0:
+            total = sum(g.double().square().sum() for g in grads).sqrt()
+            norm = total.float()
+            if max_norm > 0.0:
+                factor = (max_norm / (total + 1e-6)).clamp(max=1.0).float()
+            if skip_nonfinite and not torch.isfinite(norm):
+                return norm
+        for i, (p, g, m, v, t) in enumerate(zip(params, grads, exp_avgs, exp_avg_sqs, steps)):
+            _, lr, beta1, beta2, eps, decay = hypers[groups[i]]
+            t.add_(1)
+            count = float(t)
+            s = scales[i] if scales is not None else None
+            g = g.float() * factor
+            if s is not None:
+                numel = p.numel()
+                codes, (m, v) = (m, v), (x.reshape(-1)[:numel] for x in _decode_torch(m, v, s))
+                m, v = m.as_strided(p.shape, p.stride()), v.as_strided(p.shape, p.stride())
+            m.mul_(beta1).add_(g, alpha=1.0 - beta1)
+            v.mul_(beta2).add_(g * g * (1.0 - beta2))
+            root = math.sqrt(-math.expm1(count * math.log(beta2))) if beta2 else 1.0
+            size = lr / (-math.expm1(count * math.log(beta1)) if beta1 else 1.0)
+            w = p.float()
+            p.copy_(w - (lr * decay * w + size * (m / (v.sqrt() / root + eps))))
+            if s is not None:
+                flat = (numel,), (1,)
+                for out, new in zip((*codes, s), _encode_torch(m.as_strided(*flat), v.as_strided(*flat))):
+                    out.copy_(new)
+        return norm
+
+
+def _step(params, grads, exp_avgs, exp_avg_sqs, scales, steps, lr, betas, eps, weight_decay, max_norm, skip_nonfinite):
+    params, grads = list(params), list(grads)
+    bound = _max_norm(max_norm)
+    want = max_norm is not None
+    dev = steps.device
+    hyper = _hyper(lr, betas, eps, weight_decay, dev)
+    if steps.dtype != torch.float32 or not steps.is_contiguous() or steps.numel() != len(params):
+        raise ValueError("steps: a contiguous float32 tensor with one count per parameter")
+    if not params:
+        return torch.zeros((), device=dev) if want or skip_nonfinite else None
+    if params[0].device != dev:
+        raise ValueError("steps: on another device than the parameters")
+    if hyper[0] is not None and not dev.type == "cuda":
+        raise ValueError("lr: on another device than the parameters")
+    grads = _check(params, grads, exp_avgs, exp_avg_sqs, scales)
+    if dev.type != "cuda":
+        return _run_torch(params, grads, exp_avgs, exp_avg_sqs, scales, list(steps.view(-1)), [0] * len(params), [hyper],
+                          bound, skip_nonfinite, want)
+    base = steps.data_ptr()
+    at = array("Q", range(base, base + 4 * len(params), 4))
+    return _run(params, grads, exp_avgs, exp_avg_sqs, scales, at, array("i", bytes(4 * len(params))), [hyper], bound,
+                skip_nonfinite, want)
+
+
+def adamw_step(params, grads, exp_avgs, exp_avg_sqs, steps, *, lr, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.0,
+               max_norm=None, skip_nonfinite=False):
+    """One AdamW step, in place, of lists of tensors on one device; moments are fp32 with their parameter's shape and
+    strides, steps is fp32 [len(params)], all of it zero before the first step.  Returns the joint gradient norm (before
+    clipping; a 0-dim device tensor) with max_norm (inf: not clipped) or skip_nonfinite, else None."""
+    return _step(params, grads, exp_avgs, exp_avg_sqs, None, steps, lr, betas, eps, weight_decay, max_norm, skip_nonfinite)
+
+
+def adamw8_step(params, grads, exp_avgs, exp_avg_sqs, scales, steps, *, lr, betas=(0.9, 0.999), eps=1e-8,
+                weight_decay=0.0, max_norm=None, skip_nonfinite=False):
+    """adamw_step with 8-bit moments: of a parameter of n elements, exp_avg is int8 [ceil(n / 256), 256], exp_avg_sq uint8
+    of that shape and scales fp32 [ceil(n / 256), 2]; elements count in the order of memory."""
+    return _step(params, grads, exp_avgs, exp_avg_sqs, list(scales), steps, lr, betas, eps, weight_decay, max_norm,
+                 skip_nonfinite)
+
+
+def grad_norm(tensors):
+    """(total, each): the 2-norm of all tensors together (0-dim) and of every one ([len(tensors)]), fp32 tensors on their
+    device.  Squares and sums in 64 bits; the same bits on every run."""
+    tensors = list(tensors)
+    if not tensors:
+        raise ValueError("grad_norm: no tensors")
+    dev = tensors[0].device
+    for i, t in enumerate(tensors):
+        if t.dtype not in _DTYPES or t.layout is not torch.strided or t.device != dev:
+            raise ValueError(f"tensor {i}: dense float32, bfloat16 or float16 on the device of tensor 0 is wanted")
+    with torch.no_grad():
+        if dev.type != "cuda":
+            each = torch.stack([t.double().square().sum() for t in tensors])
+            return each.sum().sqrt().float(), each.sqrt().float()
+        tensors = [t if t.is_contiguous() or _dense(t) else t.contiguous() for t in tensors]
+        n = len(tensors)
+        grads, numels = _addresses(tensors), array("q", [t.numel() for t in tensors])
+        dtypes = array("i", [_DTYPES[t.dtype] for t in tensors])
+        L = _lib.lib()
+        with _on(dev):
+            out = torch.empty(n + 1, dtype=torch.float32, device=dev)
+            size = L.pir_grad_norm_workspace_bytes(n, _at(numels))
+            work = torch.empty(size, dtype=torch.uint8, device=dev)
+            _lib.check(L.pir_grad_norm(n, _at(grads), _at(numels), _at(dtypes), out.data_ptr(), out.data_ptr() + 4,
+                                       work.data_ptr(), size, torch.cuda.current_stream(dev).cuda_stream), "pir_grad_norm")
+    return out[0], out[1:]
+
+
+# ------------------------------------------------------------------------------------------------ 8-bit moments
+def _decode_torch(exp_avg, exp_avg_sq, scales):
+    q, c = exp_avg.float() / 127, exp_avg_sq.float() / 255
+    c = c * c
+    return scales[:, :1] * (q * q.abs()), scales[:, 1:] * (c * c)
+
+
+def _encode_torch(m, v):
+    numel = m.numel()
+    nb = _blocks(numel)
+    m, v = (torch.nn.functional.pad(x.reshape(-1).float(), (0, nb * BLOCK - numel)).view(nb, BLOCK) for x in (m, v))
+    scales = torch.stack([m.abs().amax(1), v.abs().amax(1)], 1)
+    scales = torch.where(torch.isfinite(scales), torch.where(scales < _TINY, 0.0, scales), math.nan)
+    a, b = scales[:, :1], scales[:, 1:]
+    q = torch.where(a > 0, (127 * (m.abs() / a).sqrt()).round() * m.sign(), 0.0)
+    c = torch.where((b > 0) & (v > 0), (255 * (v / b).sqrt().sqrt()).round().clamp(min=1), 0.0)
+    return q.to(torch.int8), c.to(torch.uint8), scales
+
+
+def moments8_encode(exp_avg, exp_avg_sq):
+    """Moments of one tensor (float32, bfloat16 or float16, both of one shape, strides and type) -> (int8 codes, uint8
+    codes, scales) as adamw8_step takes them."""
+    m, v = exp_avg, exp_avg_sq
+    if m.dtype not in _DTYPES or v.dtype != m.dtype or m.device != v.device or not _same_layout(m, v):
+        raise ValueError("moments: float32, bfloat16 or float16, both of one type, shape, strides and device")
+    if not _dense(m):
+        raise ValueError("moments: their elements do not fill one stretch of memory")
+    with torch.no_grad():
+        numel, nb, dev = m.numel(), _blocks(m.numel()), m.device
+        if dev.type != "cuda":
+            return _encode_torch(m.as_strided((numel,), (1,)), v.as_strided((numel,), (1,)))
+        out = (torch.empty(nb, BLOCK, dtype=torch.int8, device=dev), torch.empty(nb, BLOCK, dtype=torch.uint8, device=dev),
+               torch.empty(nb, 2, dtype=torch.float32, device=dev))
+        with _on(dev):
+            _lib.check(_lib.lib().pir_moments8_encode(numel, _DTYPES[m.dtype], m.data_ptr(), v.data_ptr(),
+                                                      *[t.data_ptr() for t in out],
+                                                      torch.cuda.current_stream(dev).cuda_stream), "pir_moments8_encode")
+        return out
+
+
+def moments8_decode(exp_avg, exp_avg_sq, scales, dtype=torch.float32):
+    """8-bit moments of any number of blocks -> (exp_avg, exp_avg_sq) as values of dtype, [blocks, 256] each."""
+    q, c, s = exp_avg, exp_avg_sq, scales
+    if dtype not in _DTYPES:
+        raise ValueError(f"dtype: {dtype} is not supported (float32, bfloat16, float16)")
+    if q.dtype != torch.int8 or c.dtype != torch.uint8 or s.dtype != torch.float32 or q.dim() != 2 or q.shape[1] != BLOCK \
+            or c.shape != q.shape or tuple(s.shape) != (q.shape[0], 2) or not (q.device == c.device == s.device) \
+            or not (q.is_contiguous() and c.is_contiguous() and s.is_contiguous()):
+        raise ValueError("moments: contiguous int8 and uint8 [blocks, 256] with float32 scales [blocks, 2] are wanted")
+    if q.device.type != "cuda":
+        return tuple(x.to(dtype) for x in _decode_torch(q, c, s))
+    if (q.data_ptr() | c.data_ptr()) % 16 or s.data_ptr() % 8:
+        raise ValueError("moments: codes have to start at a multiple of 16 bytes, scales of 8")
+    m, v = (torch.empty(q.shape, dtype=dtype, device=q.device) for _ in range(2))
+    with _on(q.device):
+        _lib.check(_lib.lib().pir_moments8_decode(q.shape[0], q.data_ptr(), c.data_ptr(), s.data_ptr(), _DTYPES[dtype],
+                                                  m.data_ptr(), v.data_ptr(),
+                                                  torch.cuda.current_stream(q.device).cuda_stream), "pir_moments8_decode")
+    return m, v
+
+
+# ------------------------------------------------------------------------------------------------- the optimizer
+class AdamW(torch.optim.Optimizer):
+    """torch.optim.AdamW's step (weight_decay=0: torch.optim.Adam's) in one call for all parameters of a device.
+
+    state_bits=8 keeps the moments of parameters of at least min_8bit_numel elements in 8 bits (2.03 bytes a parameter in
+    place of 8); smaller ones, biases above all, stay in 32.  max_norm clips the joint gradient norm of the optimizer's
+    parameters inside the step, without a pass of its own; skip_nonfinite leaves parameters, moments and step counts as
+    they are in a step whose gradients hold an infinity or a NaN.  Either leaves the norm before clipping in total_norm, a
+    device tensor.  A parameter without a gradient is skipped: no state, no step counted.
+
+    state[p]: "step" (fp32, on p's device), "exp_avg", "exp_avg_sq" and, in 8 bits, "scales".  load_state_dict takes the
+    states of torch.optim.Adam and AdamW too, and converts between 32 and 8 bits as this optimizer's groups ask for."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, min_8bit_numel=4096,
+                 max_norm=None, skip_nonfinite=False):
+        _max_norm(max_norm)
+        self.max_norm, self.skip_nonfinite, self.total_norm = max_norm, skip_nonfinite, None
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits,
+                                      min_8bit_numel=min_8bit_numel))
+
+    def add_param_group(self, param_group):
+        super().add_param_group(param_group)
+        g = self.param_groups[-1]
+        try:
+            _hyper(g["lr"], g["betas"], g["eps"], g["weight_decay"], g["params"][0].device if g["params"] else None)
+            if g["state_bits"] not in (32, 8):
+                raise ValueError(f"state_bits has to be 32 or 8: {g['state_bits']}")
+        except ValueError:
+            self.param_groups.pop()
+            raise
+
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        for g in self.param_groups:
+            for k, v in self.defaults.items():
+                g.setdefault(k, v)
+
+    @staticmethod
+    def _in_8_bits(p, group):
+        return group["state_bits"] == 8 and p.numel() >= group["min_8bit_numel"]
+
+    def _state_of(self, p, group):
+        s = self.state[p]
+        if not s:
+            s["step"] = torch.zeros((), dtype=torch.float32, device=p.device)
+            if self._in_8_bits(p, group):
+                nb = _blocks(p.numel())
+                s["exp_avg"] = torch.zeros(nb, BLOCK, dtype=torch.int8, device=p.device)
+                s["exp_avg_sq"] = torch.zeros(nb, BLOCK, dtype=torch.uint8, device=p.device)
+                s["scales"] = torch.zeros(nb, 2, dtype=torch.float32, device=p.device)
+            else:
+                for k in ("exp_avg", "exp_avg_sq"):
+                    s[k] = torch.zeros_like(p, dtype=torch.float32, requires_grad=False, memory_format=torch.preserve_format)
+        return s
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        self.total_norm = step_together([self], self.max_norm, self.skip_nonfinite)
+        return loss
+
+    def load_state_dict(self, state_dict):
+        """Takes what state_dict() of this class, torch.optim.Adam or torch.optim.AdamW returns."""
+        for g in state_dict["param_groups"]:
+            if g.get("amsgrad") or g.get("maximize"):
+                raise ValueError("amsgrad and maximize are not supported")
+            if g.get("weight_decay") and not g.get("decoupled_weight_decay", True):
+                raise ValueError("the weight decay of torch.optim.Adam (added to the gradient) is not supported")
+        saved = state_dict["state"]
+        super().load_state_dict({**state_dict, "state": {}})
+        ids = [i for g in state_dict["param_groups"] for i in g["params"]]
+        for i, (p, g) in zip(ids, [(p, g) for g in self.param_groups for p in g["params"]]):
+            if i in saved and saved[i]:
+                self._load_one(p, g, saved[i])
+
+    def _load_one(self, p, group, saved):
+        step = float(saved["step"])
+        s = self._state_of(p, group)
+        s["step"].fill_(step)
+        put = {k: saved[k].detach().to(p.device) for k in ("exp_avg", "exp_avg_sq", "scales") if k in saved}
+        if "scales" in s and "scales" not in put:
+            like = torch.empty_like(p, dtype=torch.float32, requires_grad=False)
+            m, v = (like.clone().copy_(put[k]) for k in ("exp_avg", "exp_avg_sq"))
+            put = dict(zip(("exp_avg", "exp_avg_sq", "scales"), moments8_encode(m, v)))
+        elif "scales" not in s and "scales" in put:
+            m, v = moments8_decode(*(put[k].contiguous() for k in ("exp_avg", "exp_avg_sq", "scales")))
+            put = {k: x.reshape(-1)[:p.numel()].as_strided(p.shape, p.stride()) for k, x in (("exp_avg", m), ("exp_avg_sq", v))}
+        for k, x in put.items():
+            if s[k].shape != x.shape:
+                raise ValueError(f"state {k}: {tuple(x.shape)} does not fit {tuple(s[k].shape)}")
+            s[k].copy_(x)
+
+
+@torch.no_grad()
+def step_together(optimizers, max_norm=None, skip_nonfinite=False):
+    """One step of several AdamW optimizers in one call, their gradients clipped to one joint norm.  (The optimizers' own
+    max_norm and skip_nonfinite are for their own step().)  Returns the joint norm with max_norm or skip_nonfinite."""
+    bound = _max_norm(max_norm)
+    by_device = {}
+    for opt in optimizers:
+        if not isinstance(opt, AdamW):
+            raise TypeError(f"step_together takes pir_amd.optim.AdamW optimizers, not {type(opt).__name__}")
+        for group in opt.param_groups:
+            live = [p for p in group["params"] if p.grad is not None]
+            for dev in {p.device for p in live}:
+                job = by_device.setdefault(dev, ([], [], []))
+                mine = [p for p in live if p.device == dev]
+                job[0].extend(mine)
+                job[1].extend([len(job[2])] * len(mine))
+                job[2].append((opt, group))
+    if len(by_device) > 1 and (bound or skip_nonfinite):
+        raise ValueError("a joint norm of parameters on several devices is not supported")
+    norm = torch.zeros(()) if max_norm is not None or skip_nonfinite else None      # what no gradients have
+    for dev, (params, index, owners) in by_device.items():
+        hypers = [_hyper(g["lr"], g["betas"], g["eps"], g["weight_decay"], dev) for _, g in owners]
+        if dev.type != "cuda" and any(h[0] is not None for h in hypers):
+            raise ValueError("lr: on another device than the parameters")
+        states = [owners[k][0]._state_of(p, owners[k][1]) for p, k in zip(params, index)]
+        m, v, t = ([s[k] for s in states] for k in ("exp_avg", "exp_avg_sq", "step"))
+        scales = [s.get("scales") for s in states]
+        grads = _check(params, [p.grad for p in params], m, v, scales)
+        if dev.type == "cuda":
+            norm = _run(params, grads, m, v, scales, _addresses(t), array("i", index), hypers, bound, skip_nonfinite,
+                        max_norm is not None)
+        else:
+            norm = _run_torch(params, grads, m, v, scales, t, index, hypers, bound, skip_nonfinite, max_norm is not None)
+    return norm

@@ -17,6 +17,7 @@ from typing import Dict, List, Optional
 import numpy as np
 import torch
 
+from . import optim
 from .models.image_losses import PyramidL2Loss, ssim_loss_fn
 from .renderer.raytracer import render_camera, render_camera_visibility
 
@@ -59,21 +60,44 @@ class TrainState:
     pyramidl2_loss_fn: Optional[torch.nn.Module] = None
     grad_hook: Optional[object] = None      # called between backward and the optimizer steps (data-parallel all-reduce)
     last: dict = field(default_factory=dict)
+    max_grad_norm: Optional[float] = None   # joint 2-norm the gradients of an iteration's optimizers are clipped to
 
 
-def make_optimizers(sdf_network, color_network_dict, dino_network, lr, render_visibility):
-    """render_surface.py:213-231: Adam per network; the light offset is only trainable with --render_visibility."""
-    sdf_opt = torch.optim.Adam(sdf_network.parameters(), lr=lr["sdf_network"])
+def make_optimizers(sdf_network, color_network_dict, dino_network, lr, render_visibility, optimizer="adam"):
+    """render_surface.py:213-231: Adam per network; the light offset is only trainable with --render_visibility.
+
+    optimizer: "adam" = torch.optim.Adam; "adamw" = pir_amd.optim.AdamW without weight decay (the same step), which
+    `training_step` runs for all networks in one call; "adamw8" = the same with the weights' moments in 8 bits."""
+    kinds = {"adam": torch.optim.Adam,
+             "adamw": lambda params, **k: optim.AdamW(params, weight_decay=0.0, **k),
+             "adamw8": lambda params, **k: optim.AdamW(params, weight_decay=0.0, state_bits=8, **k)}
+    if optimizer not in kinds:
+        raise ValueError(f"optimizer: one of {sorted(kinds)}, not {optimizer!r}")
+    make = kinds[optimizer]
+    sdf_opt = make(sdf_network.parameters(), lr=lr["sdf_network"])
     pl = color_network_dict["point_light_network"]
     groups = [{"params": [pl.light], "lr": 2e-5}]
     if render_visibility:
         groups.append({"params": list(pl.light_offset.parameters()), "lr": 1e-4})
     color_opts = {}
     for name, net in color_network_dict.items():
-        color_opts[name] = torch.optim.Adam(groups) if name == "point_light_network" else \
-            torch.optim.Adam(net.parameters(), lr=lr[name])
-    dino_opt = torch.optim.Adam(dino_network.parameters(), lr=lr.get("dino_network", 1e-3))
+        color_opts[name] = make(groups) if name == "point_light_network" else make(net.parameters(), lr=lr[name])
+    dino_opt = make(dino_network.parameters(), lr=lr.get("dino_network", 1e-3))
     return sdf_opt, color_opts, dino_opt
+
+
+def step_optimizers(optimizers, max_grad_norm=None):
+    """One step of each optimizer, their gradients clipped to the joint norm max_grad_norm first if it is given; returns
+    the norm before clipping then, else None.  pir_amd.optim.AdamW optimizers step together, clipping included."""
+    if optimizers and all(isinstance(opt, optim.AdamW) for opt in optimizers):
+        return optim.step_together(optimizers, max_norm=max_grad_norm)
+    norm = None
+    if max_grad_norm is not None:
+        norm = torch.nn.utils.clip_grad_norm_([p for opt in optimizers for g in opt.param_groups for p in g["params"]],
+                                              max_grad_norm)
+    for opt in optimizers:
+        opt.step()
+    return norm
 
 
 def train_visibility(state, out_dir, fill_holes=False, handle_edges=True):
@@ -191,22 +215,22 @@ def training_step(state, global_step, eik_points=None):
     if state.grad_hook is not None:
         state.grad_hook()
 
-    if sdf_optim:
-        state.sdf_optimizer.step()
+    stepped = [state.sdf_optimizer] if sdf_optim else []
     if roughness_warmup:
-        state.color_optimizer_dict["diffuse_albedo_network"].step()
-        state.color_optimizer_dict["specular_albedo_network"].step()
+        stepped += [state.color_optimizer_dict[k] for k in ("diffuse_albedo_network", "specular_albedo_network")]
     elif render_shadow:
-        state.color_optimizer_dict["point_light_network"].step()
+        stepped.append(state.color_optimizer_dict["point_light_network"])
     else:
-        for opt in state.color_optimizer_dict.values():
-            opt.step()
+        stepped += list(state.color_optimizer_dict.values())
+    grad_norm = step_optimizers(stepped, state.max_grad_norm)
 
     f = lambda t: float(t.detach().reshape(-1)[0]) if torch.is_tensor(t) else float(t)  # noqa: E731
     state.last = dict(loss=f(loss), img_loss=f(img_loss), img_l1_loss=f(img_l1), img_l2_loss=f(img_l2),
                       img_ssim_loss=f(img_ssim), eik_loss=f(eik_loss), roughrange_loss=f(roughrange_loss),
                       smoothness_loss=f(smoothness_loss), idx=idx, camera_crop=camera_crop, results=results,
                       convergent_mask=convergent_mask, render_shadow=render_shadow)
+    if grad_norm is not None:
+        state.last["grad_norm"] = f(grad_norm)
     # the float() reads above synchronised the stream: reading the accumulated tracer status costs no extra wait
     if hasattr(state.raytracer, "check_status"):
         state.raytracer.check_status()

@@ -1,0 +1,345 @@
+"""pir_amd.optim on the CPU: the torch form against 64 bits, the refusals, the optimizer class, its checkpoints, and the
+host checks of the C entry points (which come before any launch)."""
+import ctypes
+import math
+
+import pytest
+import torch
+
+import optim_util as U
+from pir_amd import optim, train
+
+SIZES = [0, 1, 2, 255, 256, 257, 1000]
+
+
+def run(p, g, m, v, s, steps, max_norm, **hyper):
+    if s is None:
+        return optim.adamw_step(p, g, m, v, steps, max_norm=max_norm, **hyper)
+    return optim.adamw8_step(p, g, m, v, s, steps, max_norm=max_norm, **hyper)
+
+
+@pytest.mark.parametrize("max_norm", [None, 1e-3, 10.0, math.inf])
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("dtype", U.TYPES)
+def test_torch_form_matches_64_bits(dtype, bits, max_norm):
+    U.check_step(run, SIZES, dtype, bits, "cpu", odd=True, max_norm=max_norm)
+
+
+def test_grad_norm_on_the_cpu():
+    g = [torch.randn(n, generator=torch.Generator().manual_seed(n)) for n in (1, 7, 300)] + [torch.zeros(0)]
+    total, each = optim.grad_norm(g)
+    assert abs(float(total) - U.norm64(g)) <= 1.001 * U.E * U.norm64(g) and each.shape == (4,) and float(each[3]) == 0.0
+
+
+def lists(n=300, bits=32, count=2):
+    p, g, m, v, s, steps = U.make([n] * count, torch.float32, bits, "cpu")
+    return dict(params=p, grads=g, exp_avgs=m, exp_avg_sqs=v, steps=steps, **({} if s is None else {"scales": s}))
+
+
+@pytest.mark.parametrize("what, change", [
+    ("a list too short", dict(grads=lambda x: x[:1])),
+    ("one gradient missing", dict(grads=lambda x: [x[0], None])),
+    ("a gradient of another type", dict(grads=lambda x: [x[0], x[1].half()])),
+    ("a gradient of another shape", dict(grads=lambda x: [x[0], x[1][:-1]])),
+    ("a sparse gradient", dict(grads=lambda x: [x[0], x[1].to_sparse()])),
+    ("a parameter of another type", dict(params=lambda x: [x[0], x[1].double()], grads=lambda x: [x[0], x[1].double()])),
+    ("a parameter with gaps", dict(params=lambda x: [x[0], torch.zeros(600)[::2]])),
+    ("a parameter that is one element, expanded", dict(params=lambda x: [x[0], torch.zeros(1).expand(300)])),
+    ("a parameter twice", dict(params=lambda x: [x[0], x[0]])),
+    ("parameters that overlap", dict(params=lambda x: (lambda b: [b[:300], b[299:599]])(torch.zeros(599)))),
+    ("a moment twice", dict(exp_avgs=lambda x: [x[1], x[1]])),
+    ("a moment of another type", dict(exp_avg_sqs=lambda x: [x[0], x[1].bfloat16()])),
+    ("a moment of another shape", dict(exp_avgs=lambda x: [x[0], x[1].view(30, 10)])),
+    ("step counts of another type", dict(steps=lambda x: x.int())),
+    ("a step count too few", dict(steps=lambda x: x[:1])),
+    ("a step count of each kind, strided", dict(steps=lambda x: torch.zeros(4)[::2])),
+    ("lr below zero", dict(lr=-1.0)), ("lr not a number", dict(lr=math.nan)), ("lr of two", dict(lr=torch.ones(2))),
+    ("beta1 of one", dict(betas=(1.0, 0.9))), ("beta2 below zero", dict(betas=(0.9, -0.1))),
+    ("eps below zero", dict(eps=-1e-8)), ("decay below zero", dict(weight_decay=-1.0)), ("decay infinite", dict(weight_decay=math.inf)),
+    ("max_norm of zero", dict(max_norm=0.0)), ("max_norm not a number", dict(max_norm=math.nan)),
+])
+def test_step_refuses(what, change):
+    args = dict(lists(), lr=1e-3)
+    before = {k: [t.clone() for t in args[k]] for k in ("params", "exp_avgs", "exp_avg_sqs")}
+    for k, f in change.items():
+        args[k] = f(args[k]) if callable(f) and k not in ("lr",) else f
+    lists_only = {k: args.pop(k) for k in ("params", "grads", "exp_avgs", "exp_avg_sqs", "steps")}
+    kept = lists(), before
+    with pytest.raises(ValueError):
+        optim.adamw_step(*lists_only.values(), **args)
+    assert all(torch.equal(a, b) for k in before for a, b in zip(kept[0][k], before[k])), what
+
+
+@pytest.mark.parametrize("what, change", [
+    ("codes of the wrong count", dict(exp_avgs=lambda x: [x[0], x[1][:1]])),
+    ("codes of the wrong type", dict(exp_avgs=lambda x: [x[0], x[1].view(torch.uint8)])),
+    ("scales of the wrong shape", dict(scales=lambda x: [x[0], x[1][:, :1]])),
+    ("scales of the wrong type", dict(scales=lambda x: [x[0], x[1].double()])),
+    ("scales too few", dict(scales=lambda x: x[:1])),
+    ("codes off their alignment", dict(exp_avgs=lambda x: [x[0], torch.zeros(513, dtype=torch.int8)[1:].view(2, 256)])),
+    ("codes with gaps", dict(exp_avg_sqs=lambda x: [x[0], torch.zeros(2, 512, dtype=torch.uint8)[:, ::2]])),
+])
+def test_8_bit_step_refuses(what, change):
+    args = lists(bits=8)
+    for k, f in change.items():
+        args[k] = f(args[k])
+    with pytest.raises(ValueError):
+        optim.adamw8_step(*(args[k] for k in ("params", "grads", "exp_avgs", "exp_avg_sqs", "scales", "steps")), lr=1e-3)
+
+
+def test_no_parameters_is_no_work():
+    assert optim.adamw_step([], [], [], [], torch.zeros(0), lr=1e-3) is None
+    assert float(optim.adamw_step([], [], [], [], torch.zeros(0), lr=1e-3, max_norm=1.0)) == 0.0
+    with pytest.raises(ValueError):
+        optim.grad_norm([])
+
+
+def test_norm_and_moments_refuse():
+    with pytest.raises(ValueError):
+        optim.grad_norm([torch.zeros(3, dtype=torch.float64)])
+    with pytest.raises(ValueError):
+        optim.grad_norm([torch.zeros(3).to_sparse()])
+    q, c, s = optim.moments8_encode(torch.randn(300), torch.rand(300))
+    for bad in ((q.view(-1), c, s), (q, c[:1], s), (q, c, s[:, :1]), (c, q, s), (q, c, s.double())):
+        with pytest.raises(ValueError):
+            optim.moments8_decode(*bad)
+    with pytest.raises(ValueError):
+        optim.moments8_decode(q, c, s, dtype=torch.float64)
+    for bad in ((torch.zeros(3), torch.zeros(4)), (torch.zeros(3), torch.zeros(3).half()),
+                (torch.zeros(3, dtype=torch.float64),) * 2, (torch.zeros(6)[::2],) * 2):
+        with pytest.raises(ValueError):
+            optim.moments8_encode(*bad)
+
+
+def test_moments8_round_trip():
+    """Half a step of the nearest code: of m = a x^2 with x in steps of 1/127 that is at most a (x + 1/254) / 127 with the
+    rounding's own square (1/254)^2 a; of v = b x^4 the same with 255 and its derivative."""
+    gen = torch.Generator().manual_seed(1)
+    m = torch.randn(10_000, generator=gen) * torch.exp(3 * torch.randn(10_000, generator=gen))
+    v = m ** 2 * torch.rand(10_000, generator=gen)
+    q, c, s = optim.moments8_encode(m, v)
+    U.assert_coded(q, c, s, m.double(), v.double(), 2 * U.E * m.double().abs(), 2 * U.E * v.double(), "encode")
+    a, b = (x.reshape(-1)[:10_000] for x in optim.moments8_decode(q, c, s))
+    top = s.repeat_interleave(256, 0)[:10_000]
+    x = (m.abs() / top[:, 0]).sqrt()
+    assert bool(((a - m).abs() <= top[:, 0] * ((x + 1 / 254) / 127 + 1 / 254 ** 2) + 1e-6 * m.abs()).all())
+    assert bool((b[v > 0] > 0).all())                  # no second moment is lost
+    y = (v / top[:, 1]) ** 0.25
+    half = torch.where(y > 1 / 255, 0.5 / 255, 1 / 255)
+    assert bool(((b - v).abs() <= top[:, 1] * ((y + half) ** 4 - (y - half).clamp(min=0) ** 4) + 1e-6 * v).all())
+
+
+def test_moments8_special_blocks():
+    m, v = torch.ones(6 * 256), torch.ones(6 * 256)
+    m[:256], v[:256] = 0.0, 0.0                         # nothing there
+    m[256:512] = 1e-39                                  # below 2^-126
+    m[512 + 7], v[768 + 9], m[1024] = math.inf, math.nan, -math.inf
+    q, c, s = optim.moments8_encode(m, v)
+    a, b = optim.moments8_decode(q, c, s)
+    assert float(a[0].abs().max()) == 0 and float(b[0].max()) == 0 and float(a[1].abs().max()) == 0 and bool((b[1] == 1).all())
+    assert bool(a[2].isnan().all()) and bool((b[2] == 1).all()) and bool(b[3].isnan().all()) and bool(a[4].isnan().all())
+    assert bool((a[5] == 1).all()) and bool((b[5] == 1).all())
+
+
+def networks(seed=0):
+    torch.manual_seed(seed)
+    return torch.nn.Sequential(torch.nn.Linear(3, 80), torch.nn.ReLU(), torch.nn.Linear(80, 90), torch.nn.ReLU(), torch.nn.Linear(90, 1))
+
+
+def train_steps(net, opt, steps, seed=0):
+    gen = torch.Generator().manual_seed(seed)
+    for _ in range(steps):
+        opt.zero_grad()
+        x = torch.randn(32, 3, generator=gen)
+        ((net(x) - x.sum(1, keepdim=True)) ** 2).mean().backward()
+        opt.step()
+
+
+def assert_moved_alike(a, b, start, lr, steps, part=1e-3):
+    """Parameters after the same steps: an fp32 step of Adam is at most about lr long and two evaluations of it agree to a
+    few 1e-5 of it, unless the gradient is rounding noise."""
+    for x, y, z in zip(a.parameters(), b.parameters(), start):
+        off = (x - y).abs() / lr
+        assert float(off.quantile(0.99)) <= part * steps, float(off.max())
+        assert not torch.equal(x, z)
+
+
+@pytest.mark.parametrize("decay", [0.0, 0.1])
+def test_class_takes_the_steps_of_torch(decay):
+    ours, theirs = networks(), networks()
+    start = [p.detach().clone() for p in ours.parameters()]
+    a = optim.AdamW(ours.parameters(), lr=1e-3, weight_decay=decay)
+    b = torch.optim.AdamW(theirs.parameters(), lr=1e-3, weight_decay=decay)
+    train_steps(ours, a, 6)
+    train_steps(theirs, b, 6)
+    assert_moved_alike(ours, theirs, start, 1e-3, 6)
+
+
+def test_class_state_and_skipped_parameters():
+    net = networks()
+    opt = optim.AdamW(net.parameters(), state_bits=8)
+    list(net.parameters())[0].grad = None
+    opt.step()
+    assert len(opt.state) == 0                           # no gradients: no state, no step counted
+    ps = list(net.parameters())
+    for p in ps[1:]:
+        p.grad = torch.ones_like(p)
+    opt.step()
+    assert ps[0] not in opt.state and len(opt.state) == len(ps) - 1 and float(opt.state[ps[1]]["step"]) == 1
+    assert opt.state[ps[2]]["exp_avg"].dtype == torch.int8 and opt.state[ps[2]]["scales"].shape == (29, 2)   # 80 x 90
+    assert opt.state[ps[1]]["exp_avg"].dtype == torch.float32 and "scales" not in opt.state[ps[1]]
+    assert opt.total_norm is None
+    opt.max_norm = 1.0
+    opt.step()
+    assert abs(float(opt.total_norm) - math.sqrt(sum(p.numel() for p in ps[1:]))) < 1e-4
+
+
+@pytest.mark.parametrize("kw", [dict(lr=-1), dict(betas=(0.9, 1.0)), dict(eps=-1), dict(weight_decay=-1), dict(state_bits=16),
+                                dict(max_norm=-1.0)])
+def test_class_refuses(kw):
+    with pytest.raises(ValueError):
+        optim.AdamW(networks().parameters(), **kw)
+
+
+def test_step_together_is_the_steps_with_one_norm():
+    nets = [networks(1), networks(2)]
+    copies = [networks(1), networks(2)]
+    for pair in (nets, copies):
+        for net in pair:
+            net(torch.randn(32, 3, generator=torch.Generator().manual_seed(3))).pow(2).mean().backward()
+    opts = [optim.AdamW(net.parameters(), lr=lr, state_bits=bits) for net, lr, bits in zip(nets, (1e-3, 1e-4), (32, 8))]
+    norm = optim.step_together(opts, max_norm=0.01)
+    total = torch.nn.utils.clip_grad_norm_([p for net in copies for p in net.parameters()], 0.01)
+    assert abs(float(norm) - float(total)) < 1e-6 * float(total)
+    for net, copy, lr, bits in zip(nets, copies, (1e-3, 1e-4), (32, 8)):
+        optim.AdamW(copy.parameters(), lr=lr, state_bits=bits).step()
+        for x, y in zip(net.parameters(), copy.parameters()):
+            assert float((x - y).abs().max()) <= 1e-3 * lr
+    with pytest.raises(ValueError):
+        optim.step_together([opts[0], opts[0]])
+    with pytest.raises(TypeError):
+        optim.step_together([torch.optim.Adam(nets[0].parameters())])
+    assert float(optim.step_together([], max_norm=1.0)) == 0.0
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("source", ["torch", 32, 8])
+def test_load_state_dict(source, bits):
+    """A run continues from the state of this class or of torch.optim.Adam as it would have without the break: to the bit in
+    32 bits and from 8 to 8, to the moments' rounding otherwise."""
+    net, other = networks(), networks()
+    make = lambda n, b: torch.optim.Adam(n.parameters(), lr=1e-3) if b == "torch" else \
+        optim.AdamW(n.parameters(), lr=1e-3, weight_decay=0.0, state_bits=b, min_8bit_numel=100)  # noqa: E731
+    first = make(net, source)
+    train_steps(net, first, 4)
+    other.load_state_dict(net.state_dict())
+    second = make(other, bits)
+    second.load_state_dict(first.state_dict())
+    assert second.param_groups[0]["lr"] == 1e-3
+    second.param_groups[0]["state_bits"] = bits
+    second.load_state_dict({**first.state_dict(), "param_groups": [{**first.state_dict()["param_groups"][0], "state_bits": bits}]})
+    start = [p.detach().clone() for p in net.parameters()]
+    train_steps(net, first, 1, seed=9)
+    train_steps(other, second, 1, seed=9)
+    for p in other.parameters():
+        assert float(second.state[p]["step"]) == 5
+        assert ("scales" in second.state[p]) == (bits == 8 and p.numel() >= 100)
+    # moments rounded to 8 bits move a step by some percent of its length
+    assert_moved_alike(net, other, start, 1e-3, 1, part=1e-3 if source != 8 and bits == 32 or source == bits else 0.3)
+    back = torch.optim.AdamW(networks().parameters(), lr=1e-3)
+    if bits == 32:
+        back.load_state_dict(second.state_dict())        # and torch takes it back
+        assert float(list(back.state.values())[0]["step"]) == 5
+
+
+def test_load_state_dict_refuses():
+    net = networks()
+    opt = optim.AdamW(net.parameters())
+    for bad in (torch.optim.Adam(net.parameters(), amsgrad=True), torch.optim.Adam(net.parameters(), weight_decay=0.1),
+                torch.optim.AdamW(net.parameters(), maximize=True)):
+        with pytest.raises(ValueError):
+            opt.load_state_dict(bad.state_dict())
+
+
+def test_skip_nonfinite_changes_nothing():
+    p, g, m, v, _, steps = U.make([300, 5], torch.float32, 32, "cpu")
+    keep = [t.clone() for x in (p, m, v) for t in x]
+    g[1][2] = math.inf
+    norm = optim.adamw_step(p, g, m, v, steps, lr=1e-3, max_norm=1.0, skip_nonfinite=True)
+    assert float(norm) == math.inf and steps.tolist() == [3.0, 4.0]
+    assert all(torch.equal(a, b) for a, b in zip(keep, [t for x in (p, m, v) for t in x]))
+
+
+def test_step_optimizers_of_a_training_run():
+    nets = {k: networks(i) for i, k in enumerate(("diffuse_albedo_network", "specular_albedo_network"))}
+
+    class Light(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.light, self.light_offset = torch.nn.Parameter(torch.tensor(1.0)), torch.nn.Linear(3, 1, bias=False)
+    nets["point_light_network"] = Light()
+    lr = {"sdf_network": 1e-5, "diffuse_albedo_network": 1e-4, "specular_albedo_network": 1e-4}
+    for kind in ("adam", "adamw", "adamw8"):
+        sdf = networks(7)
+        sdf_opt, color, dino = train.make_optimizers(sdf, nets, networks(8), lr, True, optimizer=kind)
+        assert isinstance(sdf_opt, torch.optim.Adam if kind == "adam" else optim.AdamW)
+        assert [g["lr"] for g in color["point_light_network"].param_groups] == [2e-5, 1e-4]
+        for p in sdf.parameters():
+            p.grad = torch.ones_like(p)
+        norm = train.step_optimizers([sdf_opt, color["point_light_network"]], 0.5)
+        assert abs(float(norm) - math.sqrt(sum(p.numel() for p in sdf.parameters()))) < 1e-3
+        assert train.step_optimizers([sdf_opt]) is None
+    with pytest.raises(ValueError):
+        train.make_optimizers(networks(7), nets, networks(8), lr, True, optimizer="sgd")
+
+
+def test_training_trajectory_with_adamw(monkeypatch):
+    """Five iterations of the training loop as in the trajectory test of the host logic, its optimizers exchanged for the
+    AdamW of this package: the same losses and parameters within that test's own tolerances."""
+    import functools
+    import train_traj_util
+    monkeypatch.setattr(train, "make_optimizers", functools.partial(train.make_optimizers, optimizer="adamw"))
+    out = train_traj_util.run("cpu", loss_tol=1e-4, exact_masks=False)
+    assert len(out["losses"]) >= 2
+
+
+# ---- the C entry points' host checks: every call here is refused before anything is launched
+def c_step(n=1, **change):
+    from pir_amd import _lib
+    L = _lib.lib()
+    one = (ctypes.c_void_p * 4)(*[4096] * 4)             # never read: the checks come first
+    args = dict(params=one, grads=one, m=one, v=one, scales=None, steps=one, numels=(ctypes.c_long * 4)(*[10] * 4),
+                dtypes=(ctypes.c_int * 4)(), groups=(ctypes.c_int * 4)(), group=(optim._Group * 1)(optim._Group(1e-3, 0.9, 0.99, 1e-8, 0.0, None)),
+                n_groups=1, max_norm=0.0, skip=0, norm=None, work=4096, size=0, stream=None)
+    args.update(change)
+    at = lambda x: ctypes.addressof(x) if isinstance(x, ctypes.Array) else x  # noqa: E731
+    return L.pir_adamw_step(n, *[at(x) for x in args.values()])
+
+
+@pytest.mark.parametrize("code, change", [
+    (1, dict(n=-1)), (1, dict(params=None)), (1, dict(grads=None)), (1, dict(m=None)), (1, dict(steps=None)), (1, dict(numels=None)),
+    (1, dict(groups=None)), (1, dict(group=None)), (1, dict(n_groups=0)),
+    (1, dict(numels=(ctypes.c_long * 1)(-1))), (1, dict(dtypes=(ctypes.c_int * 1)(3))), (1, dict(groups=(ctypes.c_int * 1)(1))),
+    (1, dict(grads=(ctypes.c_void_p * 1)(None))), (1, dict(params=(ctypes.c_void_p * 1)(None))), (1, dict(steps=(ctypes.c_void_p * 1)(None))),
+    (1, dict(scales=(ctypes.c_void_p * 1)(4), m=(ctypes.c_void_p * 1)(4096))),
+    (1, dict(scales=(ctypes.c_void_p * 1)(4096), m=(ctypes.c_void_p * 1)(4100))),
+    (1, dict(group=(optim._Group * 1)(optim._Group(1e-3, 1.0, 0.99, 1e-8, 0.0, None)))),
+    (1, dict(group=(optim._Group * 1)(optim._Group(math.nan, 0.9, 0.99, 1e-8, 0.0, None)))),
+    (3, dict(size=16)), (3, dict(work=None, size=1 << 20)),
+    (4, dict(numels=(ctypes.c_long * 1)(1 << 60))),
+])
+def test_c_step_refuses(code, change):
+    assert c_step(**change) == code
+
+
+def test_c_calls_without_work():
+    from pir_amd import _lib
+    L = _lib.lib()
+    assert c_step(n=0) == 0
+    assert L.pir_adamw_workspace_bytes(-1, None, 0) == 0 and L.pir_grad_norm_workspace_bytes(2, None) == 0
+    assert L.pir_moments8_decode(0, None, None, None, 0, None, None, None) == 0
+    assert L.pir_moments8_decode(1, None, None, None, 0, None, None, None) == 1
+    assert L.pir_moments8_decode(-1, None, None, None, 0, None, None, None) == 1
+    assert L.pir_moments8_encode(0, 0, None, None, None, None, None, None) == 0
+    assert L.pir_moments8_encode(5, 7, None, None, None, None, None, None) == 1
+    assert L.pir_grad_norm(1, None, None, None, None, None, None, 0, None) == 1
