@@ -1,7 +1,8 @@
-"""Build libpir_hip.so in-tree:  python -m pir_amd.build  (hipcc cross-compiles gfx950 without a GPU)."""
+"""Build libpir_hip.so and _optim_host.so in-tree:  python -m pir_amd.build  (hipcc cross-compiles gfx950 without a GPU)."""
 import os
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
@@ -10,6 +11,19 @@ SOURCES = ["sdf_eval.hip", "trace.hip", "ggx.hip", "sdf_backward.hip", "wgrad.hi
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wno-comment",
          # no packed fp32 arithmetic (v_pk_add / mul / fma_f32): its results are not reliable on this hardware
          "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+
+
+HOST_SRC = os.path.join(CSRC, "optim_host.cpp")
+HOST_OUT = os.path.join(HERE, "_optim_host.so")
+
+
+def _host_command():
+    """The extension module that reads lists of tensors for pir_amd.optim: host code against torch's C++ interface."""
+    from torch.utils import cpp_extension
+    torch_lib = cpp_extension.library_paths()[0]
+    return ([os.environ.get("CXX", "g++"), "-std=c++17", "-O2", "-fPIC", "-shared", "-I" + sysconfig.get_paths()["include"]]
+            + ["-isystem" + p for p in cpp_extension.include_paths()]
+            + [HOST_SRC, "-o", HOST_OUT, "-L" + torch_lib, "-ltorch_python", "-ltorch_cpu", "-lc10"])
 
 
 def _stale(target, deps):
@@ -36,10 +50,16 @@ def build(force=False, verbose=True):
             if verbose:
                 print(" ".join(cmd), flush=True)
             procs.append((src, subprocess.Popen(cmd)))
+    compiled = bool(procs)
+    if force or _stale(HOST_OUT, [HOST_SRC, headers[-1]]):
+        cmd = _host_command()
+        if verbose:
+            print(" ".join(cmd), flush=True)
+        procs.append(("optim_host.cpp", subprocess.Popen(cmd)))
     for src, p in procs:
         if p.wait() != 0:
-            raise RuntimeError(f"hipcc failed on {src}")
-    if force or procs or _stale(OUT, objs):
+            raise RuntimeError(f"the compiler failed on {src}")
+    if force or compiled or _stale(OUT, objs):
         cmd = [hipcc, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", OUT] + objs
         if verbose:
             print(" ".join(cmd), flush=True)

@@ -1,0 +1,223 @@
+// Host half of pir_amd.optim: reads lists of tensors into the arrays that pir_adamw_step and pir_grad_norm take, and
+// calls them.  One step of the reference's networks has some hundred tensors in each of four lists; reading their types,
+// strides and addresses through Python takes 3 us a tensor, here 0.1 us.
+//
+// Every function answers NotImplemented where the tensors are not as the kernels want them.  The Python side then says
+// what is wrong, or brings them into order and calls again.
+#include <Python.h>
+#include <ATen/ops/empty.h>
+#include <torch/csrc/autograd/python_variable.h>
+#include <algorithm>
+#include <vector>
+#include "../../include/pir_hip.h"
+
+namespace {
+
+using StepFn = decltype(&pir_adamw_step);
+using StepBytesFn = decltype(&pir_adamw_workspace_bytes);
+using NormFn = decltype(&pir_grad_norm);
+using NormBytesFn = decltype(&pir_grad_norm_workspace_bytes);
+
+// borrowed items of a list
+struct Items {
+  PyObject** at = nullptr;
+  Py_ssize_t n = -1;
+  explicit Items(PyObject* list) {
+    if (!PyList_Check(list)) return;
+    at = PySequence_Fast_ITEMS(list);
+    n = PyList_GET_SIZE(list);
+  }
+};
+
+// a plain dense tensor of this device, or null
+const at::Tensor* tensor_of(PyObject* o, c10::Device dev) {
+  if (!THPVariable_Check(o)) return nullptr;
+  const at::Tensor& t = THPVariable_Unpack(o);
+  if (!t.defined() || t.layout() != at::kStrided || t.device() != dev || t.is_neg() ||
+      t.unsafeGetTensorImpl()->is_python_dispatch())
+    return nullptr;
+  return &t;
+}
+
+int dtype_of(const at::Tensor& t) {
+  switch (t.scalar_type()) {
+    case at::kFloat: return PIR_F32;
+    case at::kBFloat16: return PIR_BF16;
+    case at::kHalf: return PIR_F16;
+    default: return -1;
+  }
+}
+
+bool same_layout(const at::Tensor& p, const at::Tensor& t) {
+  if (p.sizes() != t.sizes()) return false;
+  return p.is_contiguous() ? t.is_contiguous() : p.strides() == t.strides();
+}
+
+bool dense(const at::Tensor& t) { return t.is_contiguous() || t.is_non_overlapping_and_dense(); }
+
+char* address(const at::Tensor& t) { return (char*)t.unsafeGetTensorImpl()->mutable_data(); }
+
+// whether no byte belongs to two of the tensors; most lists are in the order of memory already
+bool disjoint(const std::vector<void*>& at, const std::vector<long>& bytes, std::vector<std::pair<char*, long>>& scratch) {
+  const size_t n = at.size();
+  char* end = nullptr;
+  size_t i = 0;
+  for (; i < n; ++i) {
+    if (bytes[i] == 0) continue;
+    if ((char*)at[i] < end) break;
+    end = (char*)at[i] + bytes[i];
+  }
+  if (i == n) return true;
+  scratch.clear();
+  for (i = 0; i < n; ++i)
+    if (bytes[i]) scratch.emplace_back((char*)at[i], bytes[i]);
+  std::sort(scratch.begin(), scratch.end());
+  for (i = 1; i < scratch.size(); ++i)
+    if (scratch[i].first < scratch[i - 1].first + scratch[i - 1].second) return false;
+  return true;
+}
+
+struct Lists {
+  std::vector<void*> p, g, m, v, s, t;
+  std::vector<long> numels, bytes, mbytes, vbytes;
+  std::vector<int> dtypes;
+};
+
+PyObject* fail(const char* what, int code) {
+  return PyErr_Format(PyExc_RuntimeError, "%s failed (code %d)", what, code);
+}
+
+// adamw_step(fn, bytes_fn, params, grads, exp_avgs, exp_avg_sqs, scales | None, steps: tensor or list, groups: array of
+// int | None, group table, n_groups, max_norm, skip_nonfinite, want_norm, device index, stream) -> norm | None
+PyObject* step(PyObject*, PyObject* args) {
+  unsigned long long fn, bytes_fn, groups_at, table, stream;
+  PyObject *params, *grads, *ms, *vs, *ss, *ts;
+  int n_groups, skip, want, index;
+  double max_norm;
+  if (!PyArg_ParseTuple(args, "KKOOOOOOKKidppiK", &fn, &bytes_fn, &params, &grads, &ms, &vs, &ss, &ts, &groups_at, &table,
+                        &n_groups, &max_norm, &skip, &want, &index, &stream))
+    return nullptr;
+  try {
+    const c10::Device dev(c10::kCUDA, (c10::DeviceIndex)index);
+    const Items P(params), G(grads), M(ms), V(vs), S(ss), T(ts);
+    const Py_ssize_t n = P.n;
+    if (n < 1 || G.n != n || M.n != n || V.n != n || (ss != Py_None && S.n != n)) Py_RETURN_NOTIMPLEMENTED;
+    Lists a;
+    for (auto* x : {&a.p, &a.g, &a.m, &a.v, &a.s, &a.t}) x->resize(n);
+    for (auto* x : {&a.numels, &a.bytes, &a.mbytes, &a.vbytes}) x->resize(n);
+    a.dtypes.resize(n);
+    for (Py_ssize_t i = 0; i < n; ++i) {
+      const at::Tensor *p = tensor_of(P.at[i], dev), *g = tensor_of(G.at[i], dev), *m = tensor_of(M.at[i], dev),
+                       *v = tensor_of(V.at[i], dev);
+      if (!p || !g || !m || !v) Py_RETURN_NOTIMPLEMENTED;
+      const long numel = p->numel();
+      const int type = dtype_of(*p);
+      if (type < 0 || g->scalar_type() != p->scalar_type() || !dense(*p) || !same_layout(*p, *g)) Py_RETURN_NOTIMPLEMENTED;
+      char *am = address(*m), *av = address(*v), *as = nullptr;
+      PyObject* so = ss == Py_None ? Py_None : S.at[i];
+      if (so == Py_None) {
+        if (m->scalar_type() != at::kFloat || v->scalar_type() != at::kFloat || !same_layout(*p, *m) || !same_layout(*p, *v))
+          Py_RETURN_NOTIMPLEMENTED;
+        a.mbytes[i] = a.vbytes[i] = 4 * numel;
+      } else {
+        const at::Tensor* s = tensor_of(so, dev);
+        const long nb = (numel + 255) / 256;
+        if (!s || s->scalar_type() != at::kFloat || m->scalar_type() != at::kChar || v->scalar_type() != at::kByte ||
+            !m->is_contiguous() || !v->is_contiguous() || !s->is_contiguous() || m->dim() != 2 || m->size(0) != nb ||
+            m->size(1) != 256 || v->sizes() != m->sizes() || s->dim() != 2 || s->size(0) != nb || s->size(1) != 2)
+          Py_RETURN_NOTIMPLEMENTED;
+        as = address(*s);
+        if ((((size_t)am | (size_t)av) & 15) || ((size_t)as & 7)) Py_RETURN_NOTIMPLEMENTED;
+        if (!as) as = (char*)16;                 // no blocks: 8-bit all the same
+        a.mbytes[i] = a.vbytes[i] = 256 * nb;
+      }
+      a.p[i] = address(*p);
+      a.g[i] = address(*g);
+      a.m[i] = am;
+      a.v[i] = av;
+      a.s[i] = as;
+      a.numels[i] = numel;
+      a.bytes[i] = numel * (long)p->element_size();
+      a.dtypes[i] = type;
+    }
+    if (T.n >= 0) {
+      if (T.n != n) Py_RETURN_NOTIMPLEMENTED;
+      for (Py_ssize_t i = 0; i < n; ++i) {
+        const at::Tensor* t = tensor_of(T.at[i], dev);
+        if (!t || t->scalar_type() != at::kFloat || t->numel() != 1) Py_RETURN_NOTIMPLEMENTED;
+        a.t[i] = address(*t);
+      }
+    } else {
+      const at::Tensor* t = tensor_of(ts, dev);
+      if (!t || t->scalar_type() != at::kFloat || t->numel() != n || !t->is_contiguous()) Py_RETURN_NOTIMPLEMENTED;
+      for (Py_ssize_t i = 0; i < n; ++i) a.t[i] = address(*t) + 4 * i;
+    }
+    std::vector<std::pair<char*, long>> scratch;
+    if (!disjoint(a.p, a.bytes, scratch) || !disjoint(a.m, a.mbytes, scratch) || !disjoint(a.v, a.vbytes, scratch))
+      Py_RETURN_NOTIMPLEMENTED;
+    std::vector<int> zeros;
+    if (!groups_at) zeros.resize(n, 0);
+    const int with_norm = want || skip || max_norm > 0.0;
+    const c10::OptionalDeviceGuard guard(dev);
+    const size_t size = ((StepBytesFn)bytes_fn)((int)n, a.numels.data(), with_norm);
+    const at::Tensor work = at::empty({(long)size}, at::TensorOptions().dtype(at::kByte).device(dev));
+    at::Tensor norm;
+    if (with_norm) norm = at::empty({}, at::TensorOptions().dtype(at::kFloat).device(dev));
+    const int code = ((StepFn)fn)((int)n, a.p.data(), (const void* const*)a.g.data(), a.m.data(), a.v.data(),
+                                  ss == Py_None ? nullptr : (float* const*)a.s.data(), (float* const*)a.t.data(),
+                                  a.numels.data(), a.dtypes.data(), groups_at ? (const int*)groups_at : zeros.data(),
+                                  (const PirAdamwGroup*)table, n_groups, max_norm, skip,
+                                  with_norm ? norm.data_ptr<float>() : nullptr, work.data_ptr(), size, (void*)stream);
+    if (code != PIR_OK) return fail("pir_adamw_step", code);
+    for (Py_ssize_t i = 0; i < n; ++i) {         // autograd and the networks' packed weights go by the version
+      const at::Tensor& p = THPVariable_Unpack(P.at[i]);
+      if (!p.is_inference()) p.unsafeGetTensorImpl()->bump_version();
+    }
+    if (!with_norm) Py_RETURN_NONE;
+    return THPVariable_Wrap(norm);
+  } catch (const std::exception& e) {
+    PyErr_SetString(PyExc_RuntimeError, e.what());
+    return nullptr;
+  }
+}
+
+// grad_norm(fn, bytes_fn, tensors, device index, stream) -> [total, norm of each]
+PyObject* norm(PyObject*, PyObject* args) {
+  unsigned long long fn, bytes_fn, stream;
+  PyObject* tensors;
+  int index;
+  if (!PyArg_ParseTuple(args, "KKOiK", &fn, &bytes_fn, &tensors, &index, &stream)) return nullptr;
+  try {
+    const c10::Device dev(c10::kCUDA, (c10::DeviceIndex)index);
+    const Items G(tensors);
+    if (G.n < 1) Py_RETURN_NOTIMPLEMENTED;
+    std::vector<void*> g(G.n);
+    std::vector<long> numels(G.n);
+    std::vector<int> dtypes(G.n);
+    for (Py_ssize_t i = 0; i < G.n; ++i) {
+      const at::Tensor* t = tensor_of(G.at[i], dev);
+      if (!t || (dtypes[i] = dtype_of(*t)) < 0 || !dense(*t)) Py_RETURN_NOTIMPLEMENTED;
+      g[i] = address(*t);
+      numels[i] = t->numel();
+    }
+    const c10::OptionalDeviceGuard guard(dev);
+    const size_t size = ((NormBytesFn)bytes_fn)((int)G.n, numels.data());
+    const at::Tensor work = at::empty({(long)size}, at::TensorOptions().dtype(at::kByte).device(dev));
+    const at::Tensor out = at::empty({G.n + 1}, at::TensorOptions().dtype(at::kFloat).device(dev));
+    float* o = out.data_ptr<float>();
+    const int code = ((NormFn)fn)((int)G.n, (const void* const*)g.data(), numels.data(), dtypes.data(), o, o + 1,
+                                  work.data_ptr(), size, (void*)stream);
+    if (code != PIR_OK) return fail("pir_grad_norm", code);
+    return THPVariable_Wrap(out);
+  } catch (const std::exception& e) {
+    PyErr_SetString(PyExc_RuntimeError, e.what());
+    return nullptr;
+  }
+}
+
+PyMethodDef methods[] = {{"adamw_step", step, METH_VARARGS, nullptr}, {"grad_norm", norm, METH_VARARGS, nullptr}, {nullptr, nullptr, 0, nullptr}};
+PyModuleDef module = {PyModuleDef_HEAD_INIT, "_optim_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
+
+}  // namespace
+
+PyMODINIT_FUNC PyInit__optim_host() { return PyModule_Create(&module); }

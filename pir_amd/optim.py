@@ -145,48 +145,41 @@ def _check(params, grads, exp_avgs, exp_avg_sqs, scales):
     return out
 
 
-def _addresses(tensors):
-    return array("Q", [0 if t is None else t.data_ptr() for t in tensors])
+_native = None
 
 
-def _at(a):
-    return a.buffer_info()[0]
-
-
-def _on(device):
-    return torch.cuda.device(device)
-
-
-def _written(tensors):
-    """The kernels write through pointers: autograd and the packed copies of the networks' weights go by the version."""
-    live = [t for t in tensors if not t.is_inference()]
-    if live:
-        torch.autograd.graph.increment_version(live)
+def _host():
+    """(module, addresses of the library's entry points).  The extension is built with the library; nothing stands in for
+    it on a GPU."""
+    global _native
+    if _native is None:
+        L = _lib.lib()
+        try:
+            from . import _optim_host
+        except ImportError as e:
+            raise _lib.PirHipError(f"pir_amd/_optim_host.so: {e}; build it first (python -m pir_amd.build)") from e
+        names = ("pir_adamw_step", "pir_adamw_workspace_bytes", "pir_grad_norm", "pir_grad_norm_workspace_bytes")
+        _native = (_optim_host, *(ctypes.cast(getattr(L, n), ctypes.c_void_p).value for n in names))
+    return _native
 
 
 def _run(params, grads, exp_avgs, exp_avg_sqs, scales, steps, groups, hypers, max_norm, skip_nonfinite, want_norm):
-    """One pir_adamw_step.  steps: addresses of the step counts; groups: index into hypers of each tensor."""
+    """One pir_adamw_step.  steps: a tensor with one count per parameter, or a list of them; groups: index into hypers of
+    each tensor, an array of int (None: all in the first)."""
     dev = params[0].device
-    n = len(params)
-    numels = array("q", [p.numel() for p in params])
-    dtypes = array("i", [_DTYPES[p.dtype] for p in params])
     table = (_Group * len(hypers))()
     for row, (dev_lr, lr, beta1, beta2, eps, decay) in zip(table, hypers):
         row.lr, row.beta1, row.beta2, row.eps, row.weight_decay = lr, beta1, beta2, eps, decay
         row.lr_device = None if dev_lr is None else dev_lr.data_ptr()
-    with_norm = want_norm or skip_nonfinite or max_norm > 0.0
-    L = _lib.lib()
-    arrays = [_addresses(x) for x in (params, grads, exp_avgs, exp_avg_sqs)]
-    arrays.append(_addresses(scales) if scales is not None else None)
-    with _on(dev):
-        norm = torch.empty((), dtype=torch.float32, device=dev) if with_norm else None
-        size = L.pir_adamw_workspace_bytes(n, _at(numels), int(with_norm))
-        work = torch.empty(size, dtype=torch.uint8, device=dev)
-        _lib.check(L.pir_adamw_step(n, *[None if a is None else _at(a) for a in arrays], _at(steps), _at(numels), _at(dtypes),
-                                    _at(groups), ctypes.addressof(table), len(hypers), max_norm, int(skip_nonfinite),
-                                    None if norm is None else norm.data_ptr(), work.data_ptr(), size,
-                                    torch.cuda.current_stream(dev).cuda_stream), "pir_adamw_step")
-    _written(params)
+    host, step, size, _, _ = _host()
+    rest = (exp_avgs, exp_avg_sqs, scales, steps, 0 if groups is None else groups.buffer_info()[0], ctypes.addressof(table),
+            len(hypers), max_norm, skip_nonfinite, want_norm, dev.index, torch.cuda.current_stream(dev).cuda_stream)
+    norm = host.adamw_step(step, size, params, grads, *rest)
+    if norm is NotImplemented:
+        grads = _check(params, grads, exp_avgs, exp_avg_sqs, scales)
+        norm = host.adamw_step(step, size, params, grads, *rest)
+        if norm is NotImplemented:
+            raise ValueError("plain tensors of one device are wanted")
     return norm
 
 
@@ -238,14 +231,11 @@ def _step(params, grads, exp_avgs, exp_avg_sqs, scales, steps, lr, betas, eps, w
         raise ValueError("steps: on another device than the parameters")
     if hyper[0] is not None and not dev.type == "cuda":
         raise ValueError("lr: on another device than the parameters")
-    grads = _check(params, grads, exp_avgs, exp_avg_sqs, scales)
     if dev.type != "cuda":
+        grads = _check(params, grads, exp_avgs, exp_avg_sqs, scales)
         return _run_torch(params, grads, exp_avgs, exp_avg_sqs, scales, list(steps.view(-1)), [0] * len(params), [hyper],
                           bound, skip_nonfinite, want)
-    base = steps.data_ptr()
-    at = array("Q", range(base, base + 4 * len(params), 4))
-    return _run(params, grads, exp_avgs, exp_avg_sqs, scales, at, array("i", bytes(4 * len(params))), [hyper], bound,
-                skip_nonfinite, want)
+    return _run(params, grads, list(exp_avgs), list(exp_avg_sqs), scales, steps, None, [hyper], bound, skip_nonfinite, want)
 
 
 def adamw_step(params, grads, exp_avgs, exp_avg_sqs, steps, *, lr, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.0,
@@ -264,6 +254,12 @@ def adamw8_step(params, grads, exp_avgs, exp_avg_sqs, scales, steps, *, lr, beta
                  skip_nonfinite)
 
 
+def _check_norm(tensors, dev):
+    for i, t in enumerate(tensors):
+        if t.dtype not in _DTYPES or t.layout is not torch.strided or t.device != dev:
+            raise ValueError(f"tensor {i}: dense float32, bfloat16 or float16 on the device of tensor 0 is wanted")
+
+
 def grad_norm(tensors):
     """(total, each): the 2-norm of all tensors together (0-dim) and of every one ([len(tensors)]), fp32 tensors on their
     device.  Squares and sums in 64 bits; the same bits on every run."""
@@ -271,24 +267,20 @@ def grad_norm(tensors):
     if not tensors:
         raise ValueError("grad_norm: no tensors")
     dev = tensors[0].device
-    for i, t in enumerate(tensors):
-        if t.dtype not in _DTYPES or t.layout is not torch.strided or t.device != dev:
-            raise ValueError(f"tensor {i}: dense float32, bfloat16 or float16 on the device of tensor 0 is wanted")
     with torch.no_grad():
         if dev.type != "cuda":
+            _check_norm(tensors, dev)
             each = torch.stack([t.double().square().sum() for t in tensors])
             return each.sum().sqrt().float(), each.sqrt().float()
-        tensors = [t if t.is_contiguous() or _dense(t) else t.contiguous() for t in tensors]
-        n = len(tensors)
-        grads, numels = _addresses(tensors), array("q", [t.numel() for t in tensors])
-        dtypes = array("i", [_DTYPES[t.dtype] for t in tensors])
-        L = _lib.lib()
-        with _on(dev):
-            out = torch.empty(n + 1, dtype=torch.float32, device=dev)
-            size = L.pir_grad_norm_workspace_bytes(n, _at(numels))
-            work = torch.empty(size, dtype=torch.uint8, device=dev)
-            _lib.check(L.pir_grad_norm(n, _at(grads), _at(numels), _at(dtypes), out.data_ptr(), out.data_ptr() + 4,
-                                       work.data_ptr(), size, torch.cuda.current_stream(dev).cuda_stream), "pir_grad_norm")
+        host, _, _, norm, size = _host()
+        stream = torch.cuda.current_stream(dev).cuda_stream
+        out = host.grad_norm(norm, size, tensors, dev.index, stream)
+        if out is NotImplemented:
+            _check_norm(tensors, dev)
+            tensors = [t.resolve_neg() if _dense(t) else t.contiguous() for t in tensors]
+            out = host.grad_norm(norm, size, tensors, dev.index, stream)
+            if out is NotImplemented:
+                raise ValueError("plain tensors of one device are wanted")
     return out[0], out[1:]
 
 
@@ -325,7 +317,7 @@ def moments8_encode(exp_avg, exp_avg_sq):
             return _encode_torch(m.as_strided((numel,), (1,)), v.as_strided((numel,), (1,)))
         out = (torch.empty(nb, BLOCK, dtype=torch.int8, device=dev), torch.empty(nb, BLOCK, dtype=torch.uint8, device=dev),
                torch.empty(nb, 2, dtype=torch.float32, device=dev))
-        with _on(dev):
+        with torch.cuda.device(dev):
             _lib.check(_lib.lib().pir_moments8_encode(numel, _DTYPES[m.dtype], m.data_ptr(), v.data_ptr(),
                                                       *[t.data_ptr() for t in out],
                                                       torch.cuda.current_stream(dev).cuda_stream), "pir_moments8_encode")
@@ -346,7 +338,7 @@ def moments8_decode(exp_avg, exp_avg_sq, scales, dtype=torch.float32):
     if (q.data_ptr() | c.data_ptr()) % 16 or s.data_ptr() % 8:
         raise ValueError("moments: codes have to start at a multiple of 16 bytes, scales of 8")
     m, v = (torch.empty(q.shape, dtype=dtype, device=q.device) for _ in range(2))
-    with _on(q.device):
+    with torch.cuda.device(q.device):
         _lib.check(_lib.lib().pir_moments8_decode(q.shape[0], q.data_ptr(), c.data_ptr(), s.data_ptr(), _DTYPES[dtype],
                                                   m.data_ptr(), v.data_ptr(),
                                                   torch.cuda.current_stream(q.device).cuda_stream), "pir_moments8_decode")
@@ -476,10 +468,10 @@ def step_together(optimizers, max_norm=None, skip_nonfinite=False):
         states = [owners[k][0]._state_of(p, owners[k][1]) for p, k in zip(params, index)]
         m, v, t = ([s[k] for s in states] for k in ("exp_avg", "exp_avg_sq", "step"))
         scales = [s.get("scales") for s in states]
-        grads = _check(params, [p.grad for p in params], m, v, scales)
+        grads = [p.grad for p in params]
         if dev.type == "cuda":
-            norm = _run(params, grads, m, v, scales, _addresses(t), array("i", index), hypers, bound, skip_nonfinite,
-                        max_norm is not None)
+            norm = _run(params, grads, m, v, scales, t, array("i", index), hypers, bound, skip_nonfinite, max_norm is not None)
         else:
+            grads = _check(params, grads, m, v, scales)
             norm = _run_torch(params, grads, m, v, scales, t, index, hypers, bound, skip_nonfinite, max_norm is not None)
     return norm

@@ -293,14 +293,28 @@ def test_step_optimizers_of_a_training_run():
         train.make_optimizers(networks(7), nets, networks(8), lr, True, optimizer="sgd")
 
 
-def test_training_trajectory_with_adamw(monkeypatch):
-    """Five iterations of the training loop as in the trajectory test of the host logic, its optimizers exchanged for the
-    AdamW of this package: the same losses and parameters within that test's own tolerances."""
+def test_training_steps_with_adamw(monkeypatch):
+    """Two iterations of the training loop with torch.optim.Adam and with this package's AdamW: the parameters they step
+    end at the same place, to a few 1e-5 of a step of lr where the gradient is no rounding noise."""
     import functools
+    import numpy as np
     import train_traj_util
-    monkeypatch.setattr(train, "make_optimizers", functools.partial(train.make_optimizers, optimizer="adamw"))
-    out = train_traj_util.run("cpu", loss_tol=1e-4, exact_masks=False)
-    assert len(out["losses"]) >= 2
+    make = train.make_optimizers
+    ends = []
+    for kind in ("adam", "adamw"):
+        monkeypatch.setattr(train, "make_optimizers", functools.partial(make, optimizer=kind))
+        d, state = train_traj_util.build_state("cpu")
+        np.random.seed(int(d["np_seed"]))
+        start = [p.detach().clone() for p in state.sdf_network.parameters()]
+        for i in range(2):
+            train.training_step(state, int(d["first_step"]) + i, eik_points=torch.from_numpy(d["eik_points"][i]))
+        ends.append(list(state.sdf_network.parameters()))
+    moved = 0
+    for x, y, z in zip(*ends, start):
+        if x.numel() >= 256 and not torch.equal(x, z):
+            moved += 1
+            assert float(((x - y).detach().abs() / 1e-5).quantile(0.95)) < 0.05
+    assert moved > 10
 
 
 # ---- the C entry points' host checks: every call here is refused before anything is launched
