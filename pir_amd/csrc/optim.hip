@@ -16,13 +16,13 @@
 namespace pir {
 
 constexpr int kOptThreads = 256;
-constexpr int kOptTable = 64;                 // tensors per launch: their descriptors travel as kernel arguments
 constexpr int kOptBlock = 256;                // elements that share a scale
-constexpr long kOptChunk = 4096;              // elements one workgroup updates
-constexpr long kNormChunk = 16384;            // elements one workgroup sums
+constexpr int kPrepRows = 52;                 // tensors and hyper-parameter sets per prologue launch: what 4 KB of kernel
+constexpr int kPrepGroups = 8;                // arguments hold
 constexpr int kPrepThreads = 1024;
-constexpr int kPrepTensors = 192;             // step counters per prologue launch
-constexpr int kPrepGroups = 16;               // hyper-parameter sets per prologue launch
+constexpr int kNormTable = 160;               // tensors per launch of the norm's first pass
+constexpr int kFinishWaves = 4;               // tensors per workgroup of the norm's second pass
+constexpr int kFirstTable = 1000;
 
 // what one tensor's update needs, computed once per step by the prologue
 struct OptCoef {
@@ -31,7 +31,9 @@ struct OptCoef {
   float gscale, run, pad0, pad1;              // clip factor; run = 0: leave the tensor as it is
 };
 
-struct OptTensor {
+// One tensor as the update kernels read it from the workspace.  The descriptors reach the device as arguments of the
+// prologue, never by a copy from host memory that a captured graph would read again at its replays.
+struct OptRow {
   void* param;
   const void* grad;
   void* m;
@@ -40,53 +42,79 @@ struct OptTensor {
   long numel;
 };
 
-struct OptTable {
-  int n;
-  const OptCoef* coef;                        // of tensor i: coef[index[i]]
-  OptTensor t[kOptTable];
-  int index[kOptTable];
-  int first[kOptTable + 1];                   // first workgroup of each tensor
+struct PrepRow {
+  OptRow row;
+  float* step;
+  unsigned first;                             // first workgroup of the tensor within its launch
+  unsigned group;
+};
+
+struct PrepGroup {
+  double lr, log1, log2, wd;
+  const float* lr_device;
+  float b1, c1, b2, c2, eps, pad;
+};
+
+struct PrepTable {
+  int n, row0, n_partial, finalize, clip, skip, n_groups, pad;
+  double max_norm;
+  const double* partial;
+  float* norm;                                // [total, clip factor]; NULL: no norm wanted
+  float* total;                               // the caller's copy of the norm, or NULL
+  OptRow* rows;
+  OptCoef* coef;
+  unsigned* first;
+  PrepGroup g[kPrepGroups];
+  PrepRow row[kPrepRows];
 };
 
 struct NormTable {
   int n;
+  unsigned chunk;                             // elements one workgroup sums
   double* partial;
-  const void* grad[kOptTable];
-  long numel[kOptTable];
-  int dtype[kOptTable];
-  int first[kOptTable + 1];
+  const void* grad[kNormTable];
+  long numel[kNormTable];                     // dtype in the lowest two bits
+  unsigned first[kNormTable];
 };
 
-struct PrepGroup {
-  double lr, log1, log2, c1, c2, wd;
-  const float* lr_device;
-  float b1, b2, eps;
-};
+struct FirstTable { int n; unsigned v[kFirstTable]; };
 
-struct PrepTable {
-  int n, n_partial, finalize, clip, skip;
-  double max_norm;
-  const double* partial;
-  float* norm;                                // [total, clip factor]
-  OptCoef* coef;
-  float* total;                               // the caller's copy of the norm, or NULL
-  float* step[kPrepTensors];
-  unsigned char group[kPrepTensors];
-  PrepGroup g[kPrepGroups];
-};
-
-static_assert(sizeof(OptTable) <= 4096 && sizeof(NormTable) <= 4096 && sizeof(PrepTable) <= 4096, "kernel arguments");
+static_assert(sizeof(PrepTable) <= 4096 && sizeof(NormTable) <= 4096 && sizeof(FirstTable) <= 4096, "kernel arguments");
 
 template <typename T> __device__ inline float to_float(T x) { return (float)x; }
 template <typename T> __device__ inline T from_float(float x) { return (T)x; }   // round to nearest even
 
-__device__ inline int find_tensor(const int* first, int n, int block) {
-  int lo = 0, hi = n;                         // first[lo] <= block < first[hi]
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (first[mid] <= block) lo = mid; else hi = mid;
+// N values of type T at any address that is a multiple of sizeof(T): one wide access all the same
+template <typename T, int N> struct Vec { typedef T type __attribute__((ext_vector_type(N), aligned(sizeof(T)))); };
+
+template <typename T, int N>
+__device__ inline void load(float (&x)[N], const T* __restrict__ p) {
+  const typename Vec<T, N>::type r = *(const typename Vec<T, N>::type*)p;
+#pragma unroll
+  for (int j = 0; j < N; ++j) x[j] = to_float(r[j]);
+}
+
+template <typename T, int N>
+__device__ inline void store(T* __restrict__ p, const float (&x)[N]) {
+  typename Vec<T, N>::type r;
+#pragma unroll
+  for (int j = 0; j < N; ++j) r[j] = from_float<T>(x[j]);
+  *(typename Vec<T, N>::type*)p = r;
+}
+
+// The last i with first[i] <= block, by a whole wave, 64 candidates at a time (first[0] = 0, ascending): two dependent
+// reads for up to 4096 tensors.
+__device__ inline int find_tensor(const unsigned* first, int n, unsigned block) {
+  const int lane = threadIdx.x & 63;
+  int lo = 0, len = n;
+  while (len > 1) {
+    const int stride = (len + 63) >> 6;
+    const bool below = lane * stride < len && first[lo + lane * stride] <= block;
+    const int part = __popcll(__ballot(below)) - 1;
+    lo += part * stride;
+    len = len - part * stride < stride ? len - part * stride : stride;
   }
-  return lo;
+  return __builtin_amdgcn_readfirstlane(lo);
 }
 
 struct Updated { float p, m, v; };
@@ -101,33 +129,87 @@ __device__ inline Updated adamw_element(const OptCoef& c, float p, float g, floa
   return r;
 }
 
+struct UpdateArgs {
+  const OptRow* rows;
+  const OptCoef* coef;
+  const unsigned* first;
+  int n;
+  unsigned chunk;                             // elements one workgroup updates, a multiple of 2048
+};
+
+// 32-bit moments: 28 bytes an element in fp32, 22 in 16 bits, bound by memory.
 template <typename T>
 __global__ void __launch_bounds__(kOptThreads)
-adamw32_kernel(const OptTable tab) {
-  const int k = find_tensor(tab.first, tab.n, blockIdx.x);
-  const OptCoef c = tab.coef[tab.index[k]];
+adamw32_kernel(const UpdateArgs args) {
+  const int k = find_tensor(args.first, args.n, blockIdx.x);
+  const OptCoef c = args.coef[k];
   if (c.run == 0.0f) return;
-  const OptTensor t = tab.t[k];
-  const long base = (long)(blockIdx.x - tab.first[k]) * kOptChunk;
-  const long end = base + kOptChunk < t.numel ? base + kOptChunk : t.numel;
+  const OptRow t = args.rows[k];
+  const long base = (long)(blockIdx.x - args.first[k]) * args.chunk;
+  const long end = base + args.chunk < t.numel ? base + args.chunk : t.numel;
   T* __restrict__ P = (T*)t.param;
   const T* __restrict__ G = (const T*)t.grad;
   float* __restrict__ M = (float*)t.m;
   float* __restrict__ V = (float*)t.v;
-  for (long i = base + threadIdx.x; i < end; i += kOptThreads) {
-    const Updated r = adamw_element(c, to_float(P[i]), to_float(G[i]), M[i], V[i]);
-    P[i] = from_float<T>(r.p);
-    M[i] = r.m;
-    V[i] = r.v;
+  auto quad = [&](float (&p)[4], const float (&g)[4], float (&m)[4], float (&v)[4]) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const Updated r = adamw_element(c, p[j], g[j], m[j], v[j]);
+      p[j] = r.p;
+      m[j] = r.m;
+      v[j] = r.v;
+    }
+  };
+  long i = base + 4 * threadIdx.x;
+  for (; i + 4 * kOptThreads + 4 <= end; i += 8 * kOptThreads) {      // two quads a thread in flight
+    float p[2][4], g[2][4], m[2][4], v[2][4];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const long at = i + h * 4 * kOptThreads;
+      load(p[h], P + at);
+      load(g[h], G + at);
+      load(m[h], M + at);
+      load(v[h], V + at);
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const long at = i + h * 4 * kOptThreads;
+      quad(p[h], g[h], m[h], v[h]);
+      store(P + at, p[h]);
+      store(M + at, m[h]);
+      store(V + at, v[h]);
+    }
   }
-}
-
-__device__ inline unsigned wave_max(unsigned x) {
-  for (int d = 32; d >= 1; d >>= 1) {
-    const unsigned y = __shfl_xor(x, d);
-    x = x > y ? x : y;
+  for (; i < end; i += 4 * kOptThreads) {     // the tensor's end
+    float p[4], g[4], m[4], v[4];
+    if (i + 4 <= end) {
+      load(p, P + i);
+      load(g, G + i);
+      load(m, M + i);
+      load(v, V + i);
+      quad(p, g, m, v);
+      store(P + i, p);
+      store(M + i, m);
+      store(V + i, v);
+      continue;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const long at = i + j < end ? i + j : i;
+      p[j] = to_float(P[at]);
+      g[j] = to_float(G[at]);
+      m[j] = M[at];
+      v[j] = V[at];
+    }
+    quad(p, g, m, v);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (i + j < end) {
+        P[i + j] = from_float<T>(p[j]);
+        M[i + j] = m[j];
+        V[i + j] = v[j];
+      }
   }
-  return x;
 }
 
 // The scale of a block from the largest bit pattern of its magnitudes: integers order like the floats they stand for,
@@ -135,6 +217,15 @@ __device__ inline unsigned wave_max(unsigned x) {
 __device__ inline float block_scale(unsigned top) {
   if (top >= 0x7f800000u) return __uint_as_float(0x7fc00000u);
   return top < 0x00800000u ? 0.0f : __uint_as_float(top);
+}
+
+__device__ inline unsigned umax(unsigned a, unsigned b) { return a > b ? a : b; }
+__device__ inline unsigned magnitude(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+
+// the largest of the 32 lanes that share a block, in all of them
+__device__ inline unsigned half_max(unsigned x) {
+  for (int d = 16; d >= 1; d >>= 1) x = umax(x, __shfl_xor(x, d));
+  return x;
 }
 
 __device__ inline float decode_m(int q, float a) { const float x = (float)q * (1.0f / 127.0f); return a * (x * fabsf(x)); }
@@ -152,47 +243,70 @@ __device__ inline int encode_v(float v, float b) {
   return c < 1 ? 1 : c;
 }
 
-// one wave per block of 256 elements, 4 consecutive ones per lane
+typedef signed char s8x8 __attribute__((ext_vector_type(8)));
+typedef unsigned char u8x8 __attribute__((ext_vector_type(8)));
+
+// 8-bit moments: half a wave per block of 256 elements, 8 consecutive ones per lane
 template <typename T>
 __global__ void __launch_bounds__(kOptThreads)
-adamw8_kernel(const OptTable tab) {
-  const int k = find_tensor(tab.first, tab.n, blockIdx.x);
-  const OptCoef c = tab.coef[tab.index[k]];
+adamw8_kernel(const UpdateArgs args) {
+  const int k = find_tensor(args.first, args.n, blockIdx.x);
+  const OptCoef c = args.coef[k];
   if (c.run == 0.0f) return;
-  const OptTensor t = tab.t[k];
-  const long base = (long)(blockIdx.x - tab.first[k]) * kOptChunk;
-  const long end = base + kOptChunk < t.numel ? base + kOptChunk : t.numel;
-  const int lane = threadIdx.x & 63;
+  const OptRow t = args.rows[k];
+  const long base = (long)(blockIdx.x - args.first[k]) * args.chunk;
+  const long end = base + args.chunk < t.numel ? base + args.chunk : t.numel;
   T* __restrict__ P = (T*)t.param;
   const T* __restrict__ G = (const T*)t.grad;
-  for (long b0 = base + (threadIdx.x >> 6) * kOptBlock; b0 < end; b0 += 4 * kOptBlock) {
-    const long i0 = b0 + 4 * lane, blk = b0 / kOptBlock;
-    char4* mq = (char4*)((signed char*)t.m + i0);
-    uchar4* vq = (uchar4*)((unsigned char*)t.v + i0);
-    const float a = t.scales[2 * blk], b = t.scales[2 * blk + 1];
-    const char4 q = *mq;
-    const uchar4 w = *vq;
-    const int qs[4] = {q.x, q.y, q.z, q.w}, ws[4] = {w.x, w.y, w.z, w.w};
-    float m[4], v[4];
+  for (long i = base + 8 * threadIdx.x; i - (i & (kOptBlock - 1)) < end; i += 8 * kOptThreads) {
+    const long blk = i / kOptBlock;
+    s8x8* mq = (s8x8*)((signed char*)t.m + i);
+    u8x8* vq = (u8x8*)((unsigned char*)t.v + i);
+    float2* sc = (float2*)t.scales + blk;
+    const s8x8 q = *mq;
+    const u8x8 w = *vq;
+    const float2 ab = *sc;
+    const bool whole = i + 8 <= end;
+    float p[8], g[8], m[8], v[8];
+    if (whole) {
+      load(p, P + i);
+      load(g, G + i);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        p[j] = i + j < end ? to_float(P[i + j]) : 0.0f;
+        g[j] = i + j < end ? to_float(G[i + j]) : 0.0f;
+      }
+    }
     unsigned ma = 0, mb = 0;
-    for (int j = 0; j < 4; ++j) {
-      m[j] = v[j] = 0.0f;                     // what fills up the last block stays zero
-      if (i0 + j >= t.numel) continue;
-      const Updated r = adamw_element(c, to_float(P[i0 + j]), to_float(G[i0 + j]), decode_m(qs[j], a), decode_v(ws[j], b));
-      P[i0 + j] = from_float<T>(r.p);
-      m[j] = r.m;
-      v[j] = r.v;
-      const unsigned x = __float_as_uint(r.m) & 0x7fffffffu, y = __float_as_uint(r.v) & 0x7fffffffu;
-      ma = ma > x ? ma : x;
-      mb = mb > y ? mb : y;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const bool in = whole || i + j < end;   // what fills up the last block stays zero
+      const Updated r = adamw_element(c, p[j], g[j], decode_m(q[j], ab.x), decode_v(w[j], ab.y));
+      p[j] = r.p;
+      m[j] = in ? r.m : 0.0f;
+      v[j] = in ? r.v : 0.0f;
+      ma = umax(ma, magnitude(m[j]));
+      mb = umax(mb, magnitude(v[j]));
     }
-    const float na = block_scale(wave_max(ma)), nb = block_scale(wave_max(mb));
-    *mq = make_char4(encode_m(m[0], na), encode_m(m[1], na), encode_m(m[2], na), encode_m(m[3], na));
-    *vq = make_uchar4(encode_v(v[0], nb), encode_v(v[1], nb), encode_v(v[2], nb), encode_v(v[3], nb));
-    if (lane == 0) {
-      t.scales[2 * blk] = na;
-      t.scales[2 * blk + 1] = nb;
+    if (whole) {
+      store(P + i, p);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (i + j < end) P[i + j] = from_float<T>(p[j]);
     }
+    const float na = block_scale(half_max(ma)), nb = block_scale(half_max(mb));
+    s8x8 nq;
+    u8x8 nw;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      nq[j] = (signed char)encode_m(m[j], na);
+      nw[j] = (unsigned char)encode_v(v[j], nb);
+    }
+    *mq = nq;
+    *vq = nw;
+    if ((threadIdx.x & 31) == 0) *sc = make_float2(na, nb);
   }
 }
 
@@ -200,42 +314,48 @@ template <typename T>
 __global__ void __launch_bounds__(kOptThreads)
 moments8_decode_kernel(long n_blocks, const signed char* __restrict__ mq, const unsigned char* __restrict__ vq,
                        const float* __restrict__ scales, T* __restrict__ m, T* __restrict__ v) {
-  const int lane = threadIdx.x & 63;
-  for (long blk = (long)blockIdx.x * 4 + (threadIdx.x >> 6); blk < n_blocks; blk += (long)gridDim.x * 4) {
-    const long i0 = blk * kOptBlock + 4 * lane;
-    const float a = scales[2 * blk], b = scales[2 * blk + 1];
-    for (int j = 0; j < 4; ++j) {
-      m[i0 + j] = from_float<T>(decode_m(mq[i0 + j], a));
-      v[i0 + j] = from_float<T>(decode_v(vq[i0 + j], b));
+  const long stride = (long)gridDim.x * kOptThreads * 8;
+  for (long i = 8 * ((long)blockIdx.x * kOptThreads + threadIdx.x); i < n_blocks * kOptBlock; i += stride) {
+    const s8x8 q = *(const s8x8*)(mq + i);
+    const u8x8 w = *(const u8x8*)(vq + i);
+    const float2 ab = ((const float2*)scales)[i / kOptBlock];
+    float x[8], y[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      x[j] = decode_m(q[j], ab.x);
+      y[j] = decode_v(w[j], ab.y);
     }
+    store(m + i, x);
+    store(v + i, y);
   }
 }
 
 template <typename T>
 __global__ void __launch_bounds__(kOptThreads)
-moments8_encode_kernel(long n_blocks, long numel, const T* __restrict__ m, const T* __restrict__ v,
-                       signed char* __restrict__ mq, unsigned char* __restrict__ vq, float* __restrict__ scales) {
-  const int lane = threadIdx.x & 63;
-  for (long blk = (long)blockIdx.x * 4 + (threadIdx.x >> 6); blk < n_blocks; blk += (long)gridDim.x * 4) {
-    const long i0 = blk * kOptBlock + 4 * lane;
-    float x[4], y[4];
+moments8_encode_kernel(long numel, const T* __restrict__ m, const T* __restrict__ v, signed char* __restrict__ mq,
+                       unsigned char* __restrict__ vq, float* __restrict__ scales) {
+  const long stride = (long)gridDim.x * kOptThreads * 8;
+  for (long i = 8 * ((long)blockIdx.x * kOptThreads + threadIdx.x); i - (i & (kOptBlock - 1)) < numel; i += stride) {
+    float x[8], y[8];
     unsigned ma = 0, mb = 0;
-    for (int j = 0; j < 4; ++j) {
-      x[j] = i0 + j < numel ? to_float(m[i0 + j]) : 0.0f;
-      y[j] = i0 + j < numel ? to_float(v[i0 + j]) : 0.0f;
-      const unsigned p = __float_as_uint(x[j]) & 0x7fffffffu, q = __float_as_uint(y[j]) & 0x7fffffffu;
-      ma = ma > p ? ma : p;
-      mb = mb > q ? mb : q;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      x[j] = i + j < numel ? to_float(m[i + j]) : 0.0f;
+      y[j] = i + j < numel ? to_float(v[i + j]) : 0.0f;
+      ma = umax(ma, magnitude(x[j]));
+      mb = umax(mb, magnitude(y[j]));
     }
-    const float a = block_scale(wave_max(ma)), b = block_scale(wave_max(mb));
-    for (int j = 0; j < 4; ++j) {
-      mq[i0 + j] = (signed char)encode_m(x[j], a);
-      vq[i0 + j] = (unsigned char)encode_v(y[j], b);
+    const float a = block_scale(half_max(ma)), b = block_scale(half_max(mb));
+    s8x8 q;
+    u8x8 w;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      q[j] = (signed char)encode_m(x[j], a);
+      w[j] = (unsigned char)encode_v(y[j], b);
     }
-    if (lane == 0) {
-      scales[2 * blk] = a;
-      scales[2 * blk + 1] = b;
-    }
+    *(s8x8*)(mq + i) = q;
+    *(u8x8*)(vq + i) = w;
+    if ((threadIdx.x & 31) == 0) ((float2*)scales)[i / kOptBlock] = make_float2(a, b);
   }
 }
 
@@ -247,53 +367,80 @@ __device__ inline double wave_sum(double x) {
   return x;
 }
 
+// 16 bytes a thread and load, four of them in flight
 template <typename T>
-__device__ inline double sum_squares(const T* __restrict__ g, long i, long end) {
-  double s = 0.0;
-  for (; i < end; i += kOptThreads) {
-    const double x = (double)to_float(g[i]);
-    s = fma(x, x, s);
+__device__ inline double sum_squares(const T* __restrict__ g, long base, long end) {
+  constexpr int N = 16 / sizeof(T);
+  constexpr long kRow = (long)N * kOptThreads;
+  double s0 = 0.0, s1 = 0.0;
+  long i = base + N * threadIdx.x;
+  for (; i + 3 * kRow + N <= end; i += 4 * kRow) {
+    float x[4][N];
+#pragma unroll
+    for (int h = 0; h < 4; ++h) load(x[h], g + i + h * kRow);
+#pragma unroll
+    for (int h = 0; h < 4; ++h)
+#pragma unroll
+      for (int j = 0; j < N; j += 2) {
+        s0 = fma((double)x[h][j], (double)x[h][j], s0);
+        s1 = fma((double)x[h][j + 1], (double)x[h][j + 1], s1);
+      }
   }
-  return s;
+  for (; i < end; i += kRow) {
+    float x[N];
+    if (i + N <= end) {
+      load(x, g + i);
+    } else {
+#pragma unroll
+      for (int j = 0; j < N; ++j) x[j] = i + j < end ? to_float(g[i + j]) : 0.0f;
+    }
+#pragma unroll
+    for (int j = 0; j < N; j += 2) {
+      s0 = fma((double)x[j], (double)x[j], s0);
+      s1 = fma((double)x[j + 1], (double)x[j + 1], s1);
+    }
+  }
+  return s0 + s1;
 }
 
 __global__ void __launch_bounds__(kOptThreads)
 norm_partial_kernel(const NormTable tab) {
   __shared__ double part[kOptThreads / 64];
   const int k = find_tensor(tab.first, tab.n, blockIdx.x);
-  const long base = (long)(blockIdx.x - tab.first[k]) * kNormChunk, numel = tab.numel[k];
-  const long end = base + kNormChunk < numel ? base + kNormChunk : numel;
-  const long i = base + threadIdx.x;
+  const long base = (long)(blockIdx.x - tab.first[k]) * tab.chunk, numel = tab.numel[k] >> 2;
+  const long end = base + tab.chunk < numel ? base + tab.chunk : numel;
+  const int dtype = tab.numel[k] & 3;
   double s;
-  if (tab.dtype[k] == PIR_F32) s = sum_squares((const float*)tab.grad[k], i, end);
-  else if (tab.dtype[k] == PIR_BF16) s = sum_squares((const __bf16*)tab.grad[k], i, end);
-  else s = sum_squares((const _Float16*)tab.grad[k], i, end);
+  if (dtype == PIR_F32) s = sum_squares((const float*)tab.grad[k], base, end);
+  else if (dtype == PIR_BF16) s = sum_squares((const __bf16*)tab.grad[k], base, end);
+  else s = sum_squares((const _Float16*)tab.grad[k], base, end);
   s = wave_sum(s);
   if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = s;
   __syncthreads();
   if (threadIdx.x == 0) tab.partial[blockIdx.x] = part[0] + part[1] + part[2] + part[3];
 }
 
-__device__ inline double block_sum(double s, double* part) {
+// sum of the partials by a workgroup of kPrepThreads
+__device__ inline double sum_partials(const double* __restrict__ partial, int n, double* part) {
+  double s = 0.0;
+  for (int i = threadIdx.x; i < n; i += kPrepThreads) s += partial[i];
   s = wave_sum(s);
   if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = s;
   __syncthreads();
   double all = 0.0;
   for (int i = 0; i < kPrepThreads / 64; ++i) all += part[i];
-  __syncthreads();
   return all;
 }
 
-// one workgroup: the joint norm and clip factor from the partial sums, then every tensor's step count and coefficients
+// One workgroup: the joint norm and clip factor from the partial sums, then the step counts and coefficients of its
+// tensors, and their descriptors for the update kernels.
 __global__ void __launch_bounds__(kPrepThreads)
 adamw_prologue_kernel(const PrepTable tab) {
   __shared__ double part[kPrepThreads / 64];
   float norm = 0.0f, clip = 1.0f;
   if (tab.norm) {
     if (tab.finalize) {
-      double s = 0.0;
-      for (int i = threadIdx.x; i < tab.n_partial; i += kPrepThreads) s += tab.partial[i];
-      const double all = sqrt(block_sum(s, part));
+      const double all = sqrt(sum_partials(tab.partial, tab.n_partial, part));
       norm = (float)all;
       if (tab.clip) {
         const double f = tab.max_norm / (all + 1e-6);
@@ -310,68 +457,86 @@ adamw_prologue_kernel(const PrepTable tab) {
     }
   }
   const bool run = !tab.skip || (norm - norm == 0.0f);
-  for (int i = threadIdx.x; i < tab.n; i += kPrepThreads) {
-    const PrepGroup& g = tab.g[tab.group[i]];
-    const float t = *tab.step[i] + 1.0f;
-    const double lr = g.lr_device ? (double)*g.lr_device : g.lr;
-    OptCoef c;
-    c.b1 = g.b1;
-    c.c1 = (float)g.c1;
-    c.b2 = g.b2;
-    c.c2 = (float)g.c2;
-    c.size = (float)(lr / -expm1((double)t * g.log1));
-    c.root = (float)(1.0 / sqrt(-expm1((double)t * g.log2)));
-    c.eps = g.eps;
-    c.decay = (float)(lr * g.wd);
-    c.gscale = clip;
-    c.run = run ? 1.0f : 0.0f;
-    c.pad0 = c.pad1 = 0.0f;
-    tab.coef[i] = c;
-    if (run) *tab.step[i] = t;
-  }
+  const int i = threadIdx.x;
+  if (i >= tab.n) return;
+  const PrepRow& r = tab.row[i];
+  const PrepGroup& g = tab.g[r.group];
+  const float t = *r.step + 1.0f;
+  const double lr = g.lr_device ? (double)*g.lr_device : g.lr;
+  OptCoef c;
+  c.b1 = g.b1;
+  c.c1 = g.c1;
+  c.b2 = g.b2;
+  c.c2 = g.c2;
+  c.size = (float)(lr / -expm1((double)t * g.log1));
+  c.root = (float)(1.0 / sqrt(-expm1((double)t * g.log2)));
+  c.eps = g.eps;
+  c.decay = (float)(lr * g.wd);
+  c.gscale = clip;
+  c.run = run ? 1.0f : 0.0f;
+  c.pad0 = c.pad1 = 0.0f;
+  tab.coef[tab.row0 + i] = c;
+  tab.rows[tab.row0 + i] = r.row;
+  tab.first[tab.row0 + i] = r.first;
+  if (run) *r.step = t;
 }
 
-// one workgroup: per-tensor norms from the partial sums of each, and the joint one
+__global__ void write_first_kernel(const FirstTable tab, unsigned* out) {
+  for (int i = threadIdx.x; i < tab.n; i += kOptThreads) out[i] = tab.v[i];
+}
+
+// norms of all tensors together (workgroup 0) and of each (a wave each, in the others), from the partial sums
 __global__ void __launch_bounds__(kPrepThreads)
-norm_finish_kernel(int n, const int* __restrict__ first, int n_partial, const double* __restrict__ partial,
+norm_finish_kernel(int n, const unsigned* __restrict__ first, int n_partial, const double* __restrict__ partial,
                    float* __restrict__ total, float* __restrict__ each) {
   __shared__ double part[kPrepThreads / 64];
-  double s = 0.0;
-  for (int i = threadIdx.x; i < n_partial; i += kPrepThreads) s += partial[i];
-  const double all = block_sum(s, part);
-  if (threadIdx.x == 0) *total = (float)sqrt(all);
-  if (each == nullptr) return;
-  for (int k = threadIdx.x >> 6; k < n; k += kPrepThreads / 64) {
-    double x = 0.0;
-    for (int i = first[k] + (threadIdx.x & 63); i < first[k + 1]; i += 64) x += partial[i];
-    x = wave_sum(x);
-    if ((threadIdx.x & 63) == 0) each[k] = (float)sqrt(x);
+  if (blockIdx.x == 0) {
+    const double all = sum_partials(partial, n_partial, part);
+    if (threadIdx.x == 0) *total = (float)sqrt(all);
+    return;
   }
-}
-
-// the prefix table of norm_finish_kernel: 256 entries at a time as kernel arguments
-struct IntTable { int n; int v[512]; };
-__global__ void write_ints_kernel(const IntTable tab, int* out) {
-  for (int i = threadIdx.x; i < tab.n; i += blockDim.x) out[i] = tab.v[i];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  if (wave >= kFinishWaves) return;
+  const int k = (blockIdx.x - 1) * kFinishWaves + wave;
+  if (k >= n) return;
+  const int end = k + 1 < n ? (int)first[k + 1] : n_partial;
+  double x = 0.0;
+  for (int i = first[k] + lane; i < end; i += 64) x += partial[i];
+  x = wave_sum(x);
+  if (lane == 0) each[k] = (float)sqrt(x);
 }
 
 static inline long ceil_div(long a, long b) { return (a + b - 1) / b; }
 
 static const long kMaxGroups = (1L << 24) - 1;     // workgroups of 256 threads: a grid has fewer than 2^32 threads
+static const long kMaxNumel = 1L << 34;            // of a tensor: what kMaxGroups of the smallest chunk reach
+static const long kMaxTotal = 1L << 36;            // of a call
 
 static int check_tensors(int n, const long* numels, const int* dtypes, const void* const* grads) {
   if (n < 0 || (n > 0 && (!numels || !dtypes || !grads))) return PIR_ERR_ARG;
+  long total = 0;
   for (int i = 0; i < n; ++i) {
     if (numels[i] < 0 || dtypes[i] < PIR_F32 || dtypes[i] > PIR_F16) return PIR_ERR_ARG;
     if (numels[i] > 0 && !grads[i]) return PIR_ERR_ARG;
-    if (ceil_div(numels[i], kOptChunk) > kMaxGroups) return PIR_ERR_TOO_LARGE;
+    if (numels[i] > kMaxNumel || (total += numels[i]) > kMaxTotal) return PIR_ERR_TOO_LARGE;
   }
   return PIR_OK;
 }
 
+// Elements a workgroup takes: as few as fill the card when there is little to do, more of them when there is much, so
+// that the search for its tensor and the second pass over the partial sums stay small beside it.
+static unsigned norm_chunk(int n, const long* numels) {
+  long total = 0;
+  for (int i = 0; i < n; ++i) total += numels[i];
+  long chunk = 4096;
+  while (chunk < 65536 && total / chunk > 4096) chunk *= 2;
+  return (unsigned)chunk;
+}
+
 static long norm_partials(int n, const long* numels) {
+  const unsigned chunk = norm_chunk(n, numels);
   long c = 0;
-  for (int i = 0; i < n; ++i) c += ceil_div(numels[i], kNormChunk);
+  for (int i = 0; i < n; ++i) c += ceil_div(numels[i], chunk);
   return c;
 }
 
@@ -379,38 +544,52 @@ static int launch_partials(int n, const void* const* grads, const long* numels, 
                            hipStream_t stream) {
   NormTable tab;
   tab.n = 0;
-  tab.first[0] = 0;
+  tab.chunk = norm_chunk(n, numels);
   tab.partial = partial;
+  long at = 0;                                  // workgroups of this launch so far
   for (int i = 0; i <= n; ++i) {
-    const long blocks = i < n ? ceil_div(numels[i], kNormChunk) : 0;
-    if (tab.n > 0 && (i == n || tab.n == kOptTable || tab.first[tab.n] + blocks > kMaxGroups)) {
-      hipLaunchKernelGGL(norm_partial_kernel, dim3(tab.first[tab.n]), dim3(kOptThreads), 0, stream, tab);
-      tab.partial += tab.first[tab.n];
+    const long blocks = i < n ? ceil_div(numels[i], tab.chunk) : 0;
+    if (tab.n > 0 && (i == n || tab.n == kNormTable || at + blocks > kMaxGroups)) {
+      hipLaunchKernelGGL(norm_partial_kernel, dim3((unsigned)at), dim3(kOptThreads), 0, stream, tab);
+      tab.partial += at;
       tab.n = 0;
+      at = 0;
     }
     if (blocks == 0) continue;
     tab.grad[tab.n] = grads[i];
-    tab.numel[tab.n] = numels[i];
-    tab.dtype[tab.n] = dtypes[i];
-    tab.first[tab.n + 1] = tab.first[tab.n] + (int)blocks;
+    tab.numel[tab.n] = numels[i] << 2 | dtypes[i];
+    tab.first[tab.n] = (unsigned)at;
+    at += blocks;
     ++tab.n;
   }
   return pir_check_launch();
 }
 
-template <int kBits>
-static void launch_update(int dtype, const OptTable& tab, hipStream_t stream) {
-  const dim3 grid(tab.first[tab.n]), block(kOptThreads);
-  if (kBits == 32) {
-    if (dtype == PIR_F32) hipLaunchKernelGGL(adamw32_kernel<float>, grid, block, 0, stream, tab);
-    else if (dtype == PIR_BF16) hipLaunchKernelGGL(adamw32_kernel<__bf16>, grid, block, 0, stream, tab);
-    else hipLaunchKernelGGL(adamw32_kernel<_Float16>, grid, block, 0, stream, tab);
-  } else {
-    if (dtype == PIR_F32) hipLaunchKernelGGL(adamw8_kernel<float>, grid, block, 0, stream, tab);
-    else if (dtype == PIR_BF16) hipLaunchKernelGGL(adamw8_kernel<__bf16>, grid, block, 0, stream, tab);
-    else hipLaunchKernelGGL(adamw8_kernel<_Float16>, grid, block, 0, stream, tab);
+static void launch_update(int kind, const UpdateArgs& args, long groups, hipStream_t stream) {
+  const dim3 grid((unsigned)groups), block(kOptThreads);
+  switch (kind) {
+    case PIR_F32: hipLaunchKernelGGL(adamw32_kernel<float>, grid, block, 0, stream, args); break;
+    case PIR_BF16: hipLaunchKernelGGL(adamw32_kernel<__bf16>, grid, block, 0, stream, args); break;
+    case PIR_F16: hipLaunchKernelGGL(adamw32_kernel<_Float16>, grid, block, 0, stream, args); break;
+    case 3 + PIR_F32: hipLaunchKernelGGL(adamw8_kernel<float>, grid, block, 0, stream, args); break;
+    case 3 + PIR_BF16: hipLaunchKernelGGL(adamw8_kernel<__bf16>, grid, block, 0, stream, args); break;
+    default: hipLaunchKernelGGL(adamw8_kernel<_Float16>, grid, block, 0, stream, args);
   }
 }
+
+static long align16(long x) { return (x + 15) & ~15L; }
+
+// the parts of a step's workspace, by their offsets
+struct StepSpace {
+  long rows, coef, first, partial, bytes;
+  StepSpace(int n, const long* numels, bool with_norm) {
+    rows = 16;                                  // [norm, clip factor, -, -] in front
+    coef = rows + (long)n * (long)sizeof(OptRow);
+    first = coef + (long)n * (long)sizeof(OptCoef);
+    partial = align16(first + 4L * n);
+    bytes = partial + (with_norm ? 8 * norm_partials(n, numels) : 0);
+  }
+};
 
 }  // namespace pir
 
@@ -420,7 +599,7 @@ extern "C" {
 
 size_t pir_adamw_workspace_bytes(int n, const long* numels, int with_norm) {
   if (n < 0 || (n > 0 && !numels)) return 0;
-  return 16 + (size_t)n * sizeof(OptCoef) + (with_norm ? 8 * (size_t)norm_partials(n, numels) : 0);
+  return (size_t)StepSpace(n, numels, with_norm != 0).bytes;
 }
 
 int pir_adamw_step(int n, void* const* params, const void* const* grads, void* const* exp_avgs, void* const* exp_avg_sqs,
@@ -442,80 +621,89 @@ int pir_adamw_step(int n, void* const* params, const void* const* grads, void* c
     if (scales && scales[i] && ((((size_t)exp_avgs[i] | (size_t)exp_avg_sqs[i]) & 15) || ((size_t)scales[i] & 7)))
       return PIR_ERR_ARG;
   }
-  const int clip = max_norm > 0.0 ? 1 : 0, with_norm = clip || skip_nonfinite || total_norm;
+  const bool clip = max_norm > 0.0, with_norm = clip || skip_nonfinite || total_norm;
   if (n == 0 && !total_norm) return PIR_OK;
-  if (!workspace || workspace_bytes < pir_adamw_workspace_bytes(n, numels, with_norm)) return PIR_ERR_SCRATCH;
-  float* norm = (float*)workspace;                                    // [total, clip factor, -, -]
-  OptCoef* coef = (OptCoef*)((char*)workspace + 16);
-  double* partial = (double*)(coef + n);
-  long n_partial = 0;
-  if (with_norm) {
-    n_partial = norm_partials(n, numels);
-    if (n_partial > 0x7fffffffL) return PIR_ERR_TOO_LARGE;
-    if (launch_partials(n, grads, numels, dtypes, partial, stream) != PIR_OK) return PIR_ERR_LAUNCH;
-  }
-  for (int i0 = 0, first = 1; first || i0 < n; first = 0) {
-    PrepTable tab;
-    tab.n = 0;
-    tab.n_partial = (int)n_partial;
-    tab.finalize = first;
-    tab.clip = clip;
-    tab.skip = skip_nonfinite != 0;
-    tab.max_norm = max_norm;
-    tab.partial = partial;
-    tab.norm = with_norm ? norm : nullptr;
-    tab.total = total_norm;
-    tab.coef = coef + i0;
-    int ids[kPrepGroups], n_ids = 0;
-    for (; i0 < n && tab.n < kPrepTensors; ++i0) {
+  const StepSpace space(n, numels, with_norm);
+  if (!workspace || workspace_bytes < (size_t)space.bytes) return PIR_ERR_SCRATCH;
+  char* ws = (char*)workspace;
+  OptRow* rows = (OptRow*)(ws + space.rows);
+  OptCoef* coef = (OptCoef*)(ws + space.coef);
+  unsigned* first = (unsigned*)(ws + space.first);
+  double* partial = (double*)(ws + space.partial);
+  long total = 0;
+  for (int i = 0; i < n; ++i) total += numels[i];
+  const unsigned chunk = total > (16L << 20) ? 8192 : 2048;
+  if (total / chunk + n > kMaxGroups) return PIR_ERR_TOO_LARGE;
+  if (with_norm && launch_partials(n, grads, numels, dtypes, partial, stream) != PIR_OK) return PIR_ERR_LAUNCH;
+
+  PrepTable tab;
+  tab.n = tab.row0 = tab.n_groups = tab.pad = 0;
+  tab.n_partial = with_norm ? (int)norm_partials(n, numels) : 0;
+  tab.finalize = 1;
+  tab.clip = clip;
+  tab.skip = skip_nonfinite != 0;
+  tab.max_norm = max_norm;
+  tab.partial = partial;
+  tab.norm = with_norm ? (float*)ws : nullptr;
+  tab.total = total_norm;
+  tab.rows = rows;
+  tab.coef = coef;
+  tab.first = first;
+  int ids[kPrepGroups];
+  auto prologue = [&]() {
+    hipLaunchKernelGGL(adamw_prologue_kernel, dim3(1), dim3(tab.norm && tab.finalize ? kPrepThreads : 64), 0, stream, tab);
+    tab.row0 += tab.n;
+    tab.n = tab.n_groups = tab.finalize = 0;
+  };
+  // tensors in the order of their kind (moments in 32 or 8 bits, then type): one update launch for each kind that occurs
+  struct { int n; long groups; } kinds[6];
+  for (int kind = 0; kind < 6; ++kind) {
+    kinds[kind].n = 0;
+    kinds[kind].groups = 0;
+    for (int i = 0; i < n; ++i) {
+      if (dtypes[i] + (scales && scales[i] ? 3 : 0) != kind) continue;
       int j = 0;
-      while (j < n_ids && ids[j] != groups[i0]) ++j;
-      if (j == n_ids) {
-        if (n_ids == kPrepGroups) break;
-        const PirAdamwGroup& g = group[groups[i0]];
-        PrepGroup& d = tab.g[n_ids];
-        ids[n_ids++] = groups[i0];
+      while (j < tab.n_groups && ids[j] != groups[i]) ++j;
+      if (tab.n == kPrepRows || (j == tab.n_groups && j == kPrepGroups)) {
+        prologue();
+        j = 0;
+      }
+      if (j == tab.n_groups) {
+        const PirAdamwGroup& g = group[groups[i]];
+        PrepGroup& d = tab.g[j];
+        ids[tab.n_groups++] = groups[i];
         d.lr = g.lr;
         d.lr_device = g.lr_device;
         d.log1 = std::log(g.beta1);
         d.log2 = std::log(g.beta2);
-        d.c1 = 1.0 - g.beta1;
-        d.c2 = 1.0 - g.beta2;
         d.wd = g.weight_decay;
         d.b1 = (float)g.beta1;
+        d.c1 = (float)(1.0 - g.beta1);
         d.b2 = (float)g.beta2;
+        d.c2 = (float)(1.0 - g.beta2);
         d.eps = (float)g.eps;
+        d.pad = 0.0f;
       }
-      tab.step[tab.n] = steps[i0];
-      tab.group[tab.n++] = (unsigned char)j;
+      PrepRow& r = tab.row[tab.n++];
+      r.row.param = params[i];
+      r.row.grad = grads[i];
+      r.row.m = exp_avgs[i];
+      r.row.v = exp_avg_sqs[i];
+      r.row.scales = kind >= 3 ? scales[i] : nullptr;
+      r.row.numel = numels[i];
+      r.step = steps[i];
+      r.first = (unsigned)kinds[kind].groups;
+      r.group = (unsigned)j;
+      kinds[kind].groups += ceil_div(numels[i], chunk);
+      ++kinds[kind].n;
     }
-    hipLaunchKernelGGL(adamw_prologue_kernel, dim3(1), dim3(kPrepThreads), 0, stream, tab);
   }
-  for (int kind = 0; kind < 6; ++kind) {                              // (8-bit moments or not) x dtype
-    const int bits8 = kind / 3, dtype = kind % 3;
-    OptTable tab;
-    tab.n = 0;
-    tab.coef = coef;
-    tab.first[0] = 0;
-    for (int i = 0; i <= n; ++i) {
-      const bool mine = i < n && dtypes[i] == dtype && (scales && scales[i] ? 1 : 0) == bits8;
-      const long blocks = mine ? ceil_div(numels[i], kOptChunk) : 0;
-      if (tab.n > 0 && (i == n || (mine && (tab.n == kOptTable || tab.first[tab.n] + blocks > kMaxGroups)))) {
-        if (bits8) launch_update<8>(dtype, tab, stream); else launch_update<32>(dtype, tab, stream);
-        tab.n = 0;
-      }
-      if (blocks == 0) continue;
-      OptTensor& t = tab.t[tab.n];
-      t.param = params[i];
-      t.grad = grads[i];
-      t.m = exp_avgs[i];
-      t.v = exp_avg_sqs[i];
-      t.scales = bits8 ? scales[i] : nullptr;
-      t.numel = numels[i];
-      tab.index[tab.n] = i;
-      tab.first[tab.n + 1] = tab.first[tab.n] + (int)blocks;
-      ++tab.n;
-    }
+  if (tab.n > 0 || tab.finalize) prologue();
+  int row = 0;
+  for (int kind = 0; kind < 6; ++kind) {
+    const UpdateArgs args = {rows + row, coef + row, first + row, kinds[kind].n, chunk};
+    if (kinds[kind].groups > 0) launch_update(kind, args, kinds[kind].groups, stream);
+    row += kinds[kind].n;
   }
   return pir_check_launch();
 }
@@ -533,32 +721,31 @@ int pir_grad_norm(int n, const void* const* grads, const long* numels, const int
   if (!total) return PIR_ERR_ARG;
   if (!workspace || workspace_bytes < pir_grad_norm_workspace_bytes(n, numels)) return PIR_ERR_SCRATCH;
   const long n_partial = norm_partials(n, numels);
-  if (n_partial > 0x7fffffffL) return PIR_ERR_TOO_LARGE;
   double* partial = (double*)workspace;
-  int* first = (int*)(partial + n_partial);
+  unsigned* first = (unsigned*)(partial + n_partial);
   if (launch_partials(n, grads, numels, dtypes, partial, stream) != PIR_OK) return PIR_ERR_LAUNCH;
   if (each) {
-    IntTable tab;
+    const unsigned chunk = norm_chunk(n, numels);
+    FirstTable tab;
     long at = 0;
     tab.n = 0;
-    int done = 0;
-    for (int i = 0; i <= n; ++i) {
-      tab.v[tab.n++] = (int)at;
-      if (i < n) at += ceil_div(numels[i], kNormChunk);
-      if (tab.n == 512 || i == n) {
-        hipLaunchKernelGGL(write_ints_kernel, dim3(1), dim3(256), 0, stream, tab, first + done);
-        done += tab.n;
+    for (int i = 0; i < n; ++i) {
+      tab.v[tab.n++] = (unsigned)at;
+      at += ceil_div(numels[i], chunk);
+      if (tab.n == kFirstTable || i == n - 1) {
+        hipLaunchKernelGGL(write_first_kernel, dim3(1), dim3(kOptThreads), 0, stream, tab, first + (i + 1 - tab.n));
         tab.n = 0;
       }
     }
   }
-  hipLaunchKernelGGL(norm_finish_kernel, dim3(1), dim3(kPrepThreads), 0, stream, n, (const int*)first, (int)n_partial,
-                     (const double*)partial, total, each);
+  const unsigned waves = each ? (unsigned)ceil_div(n, kFinishWaves) : 0;
+  hipLaunchKernelGGL(norm_finish_kernel, dim3(1 + waves), dim3(kPrepThreads), 0, stream, n, (const unsigned*)first,
+                     (int)n_partial, (const double*)partial, total, each);
   return pir_check_launch();
 }
 
 static unsigned moments8_grid(long n_blocks) {
-  const long g = (n_blocks + 3) / 4, cap = 32L * pir_num_cus();
+  const long g = ceil_div(n_blocks, 8), cap = 32L * pir_num_cus();
   return (unsigned)(g < cap ? g : cap);
 }
 
@@ -566,7 +753,8 @@ int pir_moments8_decode(long n_blocks, const signed char* exp_avg, const unsigne
                         int dtype, void* m, void* v, void* stream) {
   if (n_blocks < 0 || dtype < PIR_F32 || dtype > PIR_F16) return PIR_ERR_ARG;
   if (n_blocks == 0) return PIR_OK;
-  if (!exp_avg || !exp_avg_sq || !scales || !m || !v) return PIR_ERR_ARG;
+  if (!exp_avg || !exp_avg_sq || !scales || !m || !v || ((((size_t)exp_avg | (size_t)exp_avg_sq) & 15) || ((size_t)scales & 7)))
+    return PIR_ERR_ARG;
   const dim3 grid(moments8_grid(n_blocks)), block(kOptThreads);
   hipStream_t s = (hipStream_t)stream;
   if (dtype == PIR_F32)
@@ -582,16 +770,17 @@ int pir_moments8_encode(long numel, int dtype, const void* m, const void* v, sig
                         unsigned char* exp_avg_sq, float* scales, void* stream) {
   if (numel < 0 || dtype < PIR_F32 || dtype > PIR_F16) return PIR_ERR_ARG;
   if (numel == 0) return PIR_OK;
-  if (!exp_avg || !exp_avg_sq || !scales || !m || !v) return PIR_ERR_ARG;
+  if (!exp_avg || !exp_avg_sq || !scales || !m || !v || ((((size_t)exp_avg | (size_t)exp_avg_sq) & 15) || ((size_t)scales & 7)))
+    return PIR_ERR_ARG;
   const long n_blocks = ceil_div(numel, kOptBlock);
   const dim3 grid(moments8_grid(n_blocks)), block(kOptThreads);
   hipStream_t s = (hipStream_t)stream;
   if (dtype == PIR_F32)
-    hipLaunchKernelGGL(moments8_encode_kernel<float>, grid, block, 0, s, n_blocks, numel, (const float*)m, (const float*)v, exp_avg, exp_avg_sq, scales);
+    hipLaunchKernelGGL(moments8_encode_kernel<float>, grid, block, 0, s, numel, (const float*)m, (const float*)v, exp_avg, exp_avg_sq, scales);
   else if (dtype == PIR_BF16)
-    hipLaunchKernelGGL(moments8_encode_kernel<__bf16>, grid, block, 0, s, n_blocks, numel, (const __bf16*)m, (const __bf16*)v, exp_avg, exp_avg_sq, scales);
+    hipLaunchKernelGGL(moments8_encode_kernel<__bf16>, grid, block, 0, s, numel, (const __bf16*)m, (const __bf16*)v, exp_avg, exp_avg_sq, scales);
   else
-    hipLaunchKernelGGL(moments8_encode_kernel<_Float16>, grid, block, 0, s, n_blocks, numel, (const _Float16*)m, (const _Float16*)v, exp_avg, exp_avg_sq, scales);
+    hipLaunchKernelGGL(moments8_encode_kernel<_Float16>, grid, block, 0, s, numel, (const _Float16*)m, (const _Float16*)v, exp_avg, exp_avg_sq, scales);
   return pir_check_launch();
 }
 
