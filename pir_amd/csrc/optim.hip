@@ -222,10 +222,20 @@ __device__ inline float block_scale(unsigned top) {
 __device__ inline unsigned umax(unsigned a, unsigned b) { return a > b ? a : b; }
 __device__ inline unsigned magnitude(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 
-// the largest of the 32 lanes that share a block, in all of them
+template <int kCtrl>
+__device__ inline unsigned dpp_max(unsigned x) {
+  return umax(x, (unsigned)__builtin_amdgcn_update_dpp((int)x, (int)x, kCtrl, 0xf, 0xf, false));
+}
+
+// the largest of the 32 lanes that share a block, in all of them: lanes 1 and 2 apart, the mirrors of 8 and of 16, then
+// the two rows of 16
 __device__ inline unsigned half_max(unsigned x) {
-  for (int d = 16; d >= 1; d >>= 1) x = umax(x, __shfl_xor(x, d));
-  return x;
+  x = dpp_max<0xB1>(x);
+  x = dpp_max<0x4E>(x);
+  x = dpp_max<0x141>(x);
+  x = dpp_max<0x140>(x);
+  const auto rows = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+  return umax(rows[0], rows[1]);
 }
 
 __device__ inline float decode_m(int q, float a) { const float x = (float)q * (1.0f / 127.0f); return a * (x * fabsf(x)); }
@@ -246,7 +256,19 @@ __device__ inline int encode_v(float v, float b) {
 typedef signed char s8x8 __attribute__((ext_vector_type(8)));
 typedef unsigned char u8x8 __attribute__((ext_vector_type(8)));
 
-// 8-bit moments: half a wave per block of 256 elements, 8 consecutive ones per lane
+// 1.5 2^23: adding it to a number below 2^22 rounds that to the nearest integer, ties to even, and leaves the integer in
+// the low bits, negative ones in two's complement
+constexpr float kRoundBits = 12582912.0f;
+
+__device__ inline unsigned pack_low_bytes(float a, float b, float c, float d) {
+  const unsigned lo = __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x0c0c0400);
+  const unsigned hi = __builtin_amdgcn_perm(__float_as_uint(d), __float_as_uint(c), 0x04000c0c);
+  return lo | hi;
+}
+
+// 8-bit moments: half a wave per block of 256 elements, 8 consecutive ones per lane.  10 bytes an element (16-bit
+// parameters) leave the vector unit about 60 operations each, so the arithmetic is counted: square roots and reciprocals
+// are the hardware's (one ulp), the root of v serves the step and the new code, and codes are rounded and packed as bits.
 template <typename T>
 __global__ void __launch_bounds__(kOptThreads)
 adamw8_kernel(const UpdateArgs args) {
@@ -259,35 +281,44 @@ adamw8_kernel(const UpdateArgs args) {
   T* __restrict__ P = (T*)t.param;
   const T* __restrict__ G = (const T*)t.grad;
   for (long i = base + 8 * threadIdx.x; i - (i & (kOptBlock - 1)) < end; i += 8 * kOptThreads) {
-    const long blk = i / kOptBlock;
-    s8x8* mq = (s8x8*)((signed char*)t.m + i);
-    u8x8* vq = (u8x8*)((unsigned char*)t.v + i);
-    float2* sc = (float2*)t.scales + blk;
-    const s8x8 q = *mq;
-    const u8x8 w = *vq;
+    uint2* mq = (uint2*)((signed char*)t.m + i);
+    uint2* vq = (uint2*)((unsigned char*)t.v + i);
+    float2* sc = (float2*)t.scales + i / kOptBlock;
+    uint2 q = *mq, w = *vq;
     const float2 ab = *sc;
     const bool whole = i + 8 <= end;
-    float p[8], g[8], m[8], v[8];
+    float p[8], g[8], m[8], r[8];
     if (whole) {
       load(p, P + i);
       load(g, G + i);
-    } else {
+    } else {                                  // what fills up the last block is zero, and stays so
+      unsigned long keep = i < end ? (1ul << (8 * (end - i))) - 1 : 0;
+      q.x &= (unsigned)keep;
+      q.y &= (unsigned)(keep >> 32);
+      w.x &= (unsigned)keep;
+      w.y &= (unsigned)(keep >> 32);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         p[j] = i + j < end ? to_float(P[i + j]) : 0.0f;
         g[j] = i + j < end ? to_float(G[i + j]) : 0.0f;
       }
     }
-    unsigned ma = 0, mb = 0;
+    const float a1 = c.b1 * ab.x, b2 = c.b2 * ab.y;
+    float ma = 0.0f;
+    unsigned mb = 0;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const bool in = whole || i + j < end;   // what fills up the last block stays zero
-      const Updated r = adamw_element(c, p[j], g[j], decode_m(q[j], ab.x), decode_v(w[j], ab.y));
-      p[j] = r.p;
-      m[j] = in ? r.m : 0.0f;
-      v[j] = in ? r.v : 0.0f;
-      ma = umax(ma, magnitude(m[j]));
-      mb = umax(mb, magnitude(v[j]));
+      const int qj = (int)((j < 4 ? q.x : q.y) << (24 - 8 * (j & 3))) >> 24;
+      const unsigned wj = ((j < 4 ? w.x : w.y) >> (8 * (j & 3))) & 255u;
+      const float x = (float)qj * (1.0f / 127.0f), y = (float)wj * (1.0f / 255.0f), y2 = y * y;
+      const float gj = g[j] * c.gscale;
+      m[j] = fmaf(a1, x * fabsf(x), c.c1 * gj);
+      const float v = fmaf(b2, y2 * y2, c.c2 * gj * gj);
+      r[j] = __builtin_amdgcn_sqrtf(v);
+      const float u = m[j] * __builtin_amdgcn_rcpf(fmaf(r[j], c.root, c.eps));
+      p[j] -= fmaf(c.decay, p[j], c.size * u);
+      ma = fmaxf(ma, fabsf(m[j]));
+      mb = umax(mb, __float_as_uint(v));      // v is not below zero: its bits order as it does, NaN on top
     }
     if (whole) {
       store(P + i, p);
@@ -296,16 +327,21 @@ adamw8_kernel(const UpdateArgs args) {
       for (int j = 0; j < 8; ++j)
         if (i + j < end) P[i + j] = from_float<T>(p[j]);
     }
-    const float na = block_scale(half_max(ma)), nb = block_scale(half_max(mb));
-    s8x8 nq;
-    u8x8 nw;
+    const float nb = block_scale(half_max(mb));
+    float na = block_scale(half_max(__float_as_uint(ma)));
+    na = nb != nb ? nb : na;                  // the maximum of floats passes over a NaN, which v has too
+    const float ra = na > 0.0f ? 1.0f / na : 0.0f, rb = nb > 0.0f ? __builtin_amdgcn_rsqf(nb) : 0.0f;
+    const float live = nb > 0.0f ? 0x1p127f : 0.0f;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      nq[j] = (signed char)encode_m(m[j], na);
-      nw[j] = (unsigned char)encode_v(v[j], nb);
+      const float x = copysignf(__builtin_amdgcn_sqrtf(fabsf(m[j]) * ra), m[j]);
+      const float y = __builtin_amdgcn_sqrtf(r[j] * rb);
+      const float least = __builtin_amdgcn_fmed3f(r[j] * live, 0.0f, 1.0f / 255.0f);   // c >= 1 if v > 0: no
+      m[j] = fmaf(x, 127.0f, kRoundBits);                                              // denominator is lost
+      r[j] = fmaf(fmaxf(y, least), 255.0f, kRoundBits);
     }
-    *mq = nq;
-    *vq = nw;
+    *mq = make_uint2(pack_low_bytes(m[0], m[1], m[2], m[3]), pack_low_bytes(m[4], m[5], m[6], m[7]));
+    *vq = make_uint2(pack_low_bytes(r[0], r[1], r[2], r[3]), pack_low_bytes(r[4], r[5], r[6], r[7]));
     if ((threadIdx.x & 31) == 0) *sc = make_float2(na, nb);
   }
 }
