@@ -17,9 +17,12 @@ namespace pir {
 
 constexpr int kOptThreads = 256;
 constexpr int kOptBlock = 256;                // elements that share a scale
+constexpr int kOptChunk = 1024;               // elements one workgroup updates, with 32-bit moments
+constexpr int kOptChunk8 = 2048;              // and with 8-bit ones
 constexpr int kPrepRows = 52;                 // tensors and hyper-parameter sets per prologue launch: what 4 KB of kernel
 constexpr int kPrepGroups = 8;                // arguments hold
 constexpr int kPrepThreads = 1024;
+constexpr int kNormThreads = 1024;
 constexpr int kNormTable = 160;               // tensors per launch of the norm's first pass
 constexpr int kFinishWaves = 4;               // tensors per workgroup of the norm's second pass
 constexpr int kFirstTable = 1000;
@@ -87,19 +90,22 @@ template <typename T> __device__ inline T from_float(float x) { return (T)x; }  
 // N values of type T at any address that is a multiple of sizeof(T): one wide access all the same
 template <typename T, int N> struct Vec { typedef T type __attribute__((ext_vector_type(N), aligned(sizeof(T)))); };
 
-template <typename T, int N>
+// kStream: data that is too much for the last-level cache passes it by
+template <bool kStream, typename T, int N>
 __device__ inline void load(float (&x)[N], const T* __restrict__ p) {
-  const typename Vec<T, N>::type r = *(const typename Vec<T, N>::type*)p;
+  const typename Vec<T, N>::type* q = (const typename Vec<T, N>::type*)p;
+  const typename Vec<T, N>::type r = kStream ? __builtin_nontemporal_load(q) : *q;
 #pragma unroll
   for (int j = 0; j < N; ++j) x[j] = to_float(r[j]);
 }
 
-template <typename T, int N>
+template <bool kStream, typename T, int N>
 __device__ inline void store(T* __restrict__ p, const float (&x)[N]) {
+  typename Vec<T, N>::type* q = (typename Vec<T, N>::type*)p;
   typename Vec<T, N>::type r;
 #pragma unroll
   for (int j = 0; j < N; ++j) r[j] = from_float<T>(x[j]);
-  *(typename Vec<T, N>::type*)p = r;
+  if (kStream) __builtin_nontemporal_store(r, q); else *q = r;
 }
 
 // The last i with first[i] <= block, by a whole wave, 64 candidates at a time (first[0] = 0, ascending): two dependent
@@ -134,81 +140,66 @@ struct UpdateArgs {
   const OptCoef* coef;
   const unsigned* first;
   int n;
-  unsigned chunk;                             // elements one workgroup updates, a multiple of 2048
 };
 
-// 32-bit moments: 28 bytes an element in fp32, 22 in 16 bits, bound by memory.
-template <typename T>
+// 32-bit moments: 28 bytes an element in fp32, 22 in 16 bits, bound by memory.  A workgroup has two groups of 4
+// consecutive elements a thread, all of whose loads are in flight before the first is used.
+template <typename T, bool kStream>
 __global__ void __launch_bounds__(kOptThreads)
 adamw32_kernel(const UpdateArgs args) {
   const int k = find_tensor(args.first, args.n, blockIdx.x);
   const OptCoef c = args.coef[k];
   if (c.run == 0.0f) return;
   const OptRow t = args.rows[k];
-  const long base = (long)(blockIdx.x - args.first[k]) * args.chunk;
-  const long end = base + args.chunk < t.numel ? base + args.chunk : t.numel;
+  const long base = (long)(blockIdx.x - args.first[k]) * kOptChunk, end = t.numel;
   T* __restrict__ P = (T*)t.param;
   const T* __restrict__ G = (const T*)t.grad;
   float* __restrict__ M = (float*)t.m;
   float* __restrict__ V = (float*)t.v;
-  auto quad = [&](float (&p)[4], const float (&g)[4], float (&m)[4], float (&v)[4]) {
+  constexpr int kQuads = kOptChunk / (4 * kOptThreads);
+  float p[kQuads][4], g[kQuads][4], m[kQuads][4], v[kQuads][4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const Updated r = adamw_element(c, p[j], g[j], m[j], v[j]);
-      p[j] = r.p;
-      m[j] = r.m;
-      v[j] = r.v;
-    }
-  };
-  long i = base + 4 * threadIdx.x;
-  for (; i + 4 * kOptThreads + 4 <= end; i += 8 * kOptThreads) {      // two quads a thread in flight
-    float p[2][4], g[2][4], m[2][4], v[2][4];
+  for (int h = 0; h < kQuads; ++h) {
+    const long i = base + 4 * (h * kOptThreads + threadIdx.x);
+    if (i + 4 <= end) {
+      load<kStream>(p[h], P + i);
+      load<kStream>(g[h], G + i);
+      load<kStream>(m[h], M + i);
+      load<kStream>(v[h], V + i);
+    } else {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const long at = i + h * 4 * kOptThreads;
-      load(p[h], P + at);
-      load(g[h], G + at);
-      load(m[h], M + at);
-      load(v[h], V + at);
-    }
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const long at = i + h * 4 * kOptThreads;
-      quad(p[h], g[h], m[h], v[h]);
-      store(P + at, p[h]);
-      store(M + at, m[h]);
-      store(V + at, v[h]);
+      for (int j = 0; j < 4; ++j) {
+        const bool in = i + j < end;
+        p[h][j] = in ? to_float(P[i + j]) : 0.0f;
+        g[h][j] = in ? to_float(G[i + j]) : 0.0f;
+        m[h][j] = in ? M[i + j] : 0.0f;
+        v[h][j] = in ? V[i + j] : 0.0f;
+      }
     }
   }
-  for (; i < end; i += 4 * kOptThreads) {     // the tensor's end
-    float p[4], g[4], m[4], v[4];
-    if (i + 4 <= end) {
-      load(p, P + i);
-      load(g, G + i);
-      load(m, M + i);
-      load(v, V + i);
-      quad(p, g, m, v);
-      store(P + i, p);
-      store(M + i, m);
-      store(V + i, v);
-      continue;
-    }
+#pragma unroll
+  for (int h = 0; h < kQuads; ++h) {
+    const long i = base + 4 * (h * kOptThreads + threadIdx.x);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const long at = i + j < end ? i + j : i;
-      p[j] = to_float(P[at]);
-      g[j] = to_float(G[at]);
-      m[j] = M[at];
-      v[j] = V[at];
+      const Updated r = adamw_element(c, p[h][j], g[h][j], m[h][j], v[h][j]);
+      p[h][j] = r.p;
+      m[h][j] = r.m;
+      v[h][j] = r.v;
     }
-    quad(p, g, m, v);
+    if (i + 4 <= end) {
+      store<kStream>(P + i, p[h]);
+      store<kStream>(M + i, m[h]);
+      store<kStream>(V + i, v[h]);
+    } else {
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (i + j < end) {
-        P[i + j] = from_float<T>(p[j]);
-        M[i + j] = m[j];
-        V[i + j] = v[j];
-      }
+      for (int j = 0; j < 4; ++j)
+        if (i + j < end) {
+          P[i + j] = from_float<T>(p[h][j]);
+          M[i + j] = m[h][j];
+          V[i + j] = v[h][j];
+        }
+    }
   }
 }
 
@@ -253,6 +244,7 @@ __device__ inline int encode_v(float v, float b) {
   return c < 1 ? 1 : c;
 }
 
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 typedef signed char s8x8 __attribute__((ext_vector_type(8)));
 typedef unsigned char u8x8 __attribute__((ext_vector_type(8)));
 
@@ -269,130 +261,134 @@ __device__ inline unsigned pack_low_bytes(float a, float b, float c, float d) {
 // 8-bit moments: half a wave per block of 256 elements, 8 consecutive ones per lane.  10 bytes an element (16-bit
 // parameters) leave the vector unit about 60 operations each, so the arithmetic is counted: square roots and reciprocals
 // are the hardware's (one ulp), the root of v serves the step and the new code, and codes are rounded and packed as bits.
-template <typename T>
+template <typename T, bool kStream>
 __global__ void __launch_bounds__(kOptThreads)
 adamw8_kernel(const UpdateArgs args) {
+  static_assert(kOptChunk8 == 8 * kOptThreads, "8 elements a thread");
   const int k = find_tensor(args.first, args.n, blockIdx.x);
   const OptCoef c = args.coef[k];
   if (c.run == 0.0f) return;
   const OptRow t = args.rows[k];
-  const long base = (long)(blockIdx.x - args.first[k]) * args.chunk;
-  const long end = base + args.chunk < t.numel ? base + args.chunk : t.numel;
+  const long end = t.numel, i = (long)(blockIdx.x - args.first[k]) * kOptChunk8 + 8 * threadIdx.x;
   T* __restrict__ P = (T*)t.param;
   const T* __restrict__ G = (const T*)t.grad;
-  for (long i = base + 8 * threadIdx.x; i - (i & (kOptBlock - 1)) < end; i += 8 * kOptThreads) {
-    uint2* mq = (uint2*)((signed char*)t.m + i);
-    uint2* vq = (uint2*)((unsigned char*)t.v + i);
-    float2* sc = (float2*)t.scales + i / kOptBlock;
-    uint2 q = *mq, w = *vq;
-    const float2 ab = *sc;
-    const bool whole = i + 8 <= end;
-    float p[8], g[8], m[8], r[8];
-    if (whole) {
-      load(p, P + i);
-      load(g, G + i);
-    } else {                                  // what fills up the last block is zero, and stays so
-      unsigned long keep = i < end ? (1ul << (8 * (end - i))) - 1 : 0;
-      q.x &= (unsigned)keep;
-      q.y &= (unsigned)(keep >> 32);
-      w.x &= (unsigned)keep;
-      w.y &= (unsigned)(keep >> 32);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        p[j] = i + j < end ? to_float(P[i + j]) : 0.0f;
-        g[j] = i + j < end ? to_float(G[i + j]) : 0.0f;
-      }
-    }
-    const float a1 = c.b1 * ab.x, b2 = c.b2 * ab.y;
-    float ma = 0.0f;
-    unsigned mb = 0;
+  if (i - (i & (kOptBlock - 1)) >= end) return;       // no such block
+  u32x2* mq = (u32x2*)((signed char*)t.m + i);
+  u32x2* vq = (u32x2*)((unsigned char*)t.v + i);
+  float2* sc = (float2*)t.scales + i / kOptBlock;
+  u32x2 q = kStream ? __builtin_nontemporal_load(mq) : *mq, w = kStream ? __builtin_nontemporal_load(vq) : *vq;
+  const float2 ab = *sc;
+  const bool whole = i + 8 <= end;
+  float p[8], g[8], m[8], r[8];
+  if (whole) {
+    load<kStream>(p, P + i);
+    load<kStream>(g, G + i);
+  } else {                                  // what fills up the last block is zero, and stays so
+    unsigned long keep = i < end ? (1ul << (8 * (end - i))) - 1 : 0;
+    q.x &= (unsigned)keep;
+    q.y &= (unsigned)(keep >> 32);
+    w.x &= (unsigned)keep;
+    w.y &= (unsigned)(keep >> 32);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const int qj = (int)((j < 4 ? q.x : q.y) << (24 - 8 * (j & 3))) >> 24;
-      const unsigned wj = ((j < 4 ? w.x : w.y) >> (8 * (j & 3))) & 255u;
-      const float x = (float)qj * (1.0f / 127.0f), y = (float)wj * (1.0f / 255.0f), y2 = y * y;
-      const float gj = g[j] * c.gscale;
-      m[j] = fmaf(a1, x * fabsf(x), c.c1 * gj);
-      const float v = fmaf(b2, y2 * y2, c.c2 * gj * gj);
-      r[j] = __builtin_amdgcn_sqrtf(v);
-      const float u = m[j] * __builtin_amdgcn_rcpf(fmaf(r[j], c.root, c.eps));
-      p[j] -= fmaf(c.decay, p[j], c.size * u);
-      ma = fmaxf(ma, fabsf(m[j]));
-      mb = umax(mb, __float_as_uint(v));      // v is not below zero: its bits order as it does, NaN on top
+      p[j] = i + j < end ? to_float(P[i + j]) : 0.0f;
+      g[j] = i + j < end ? to_float(G[i + j]) : 0.0f;
     }
-    if (whole) {
-      store(P + i, p);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (i + j < end) P[i + j] = from_float<T>(p[j]);
-    }
-    const float nb = block_scale(half_max(mb));
-    float na = block_scale(half_max(__float_as_uint(ma)));
-    na = nb != nb ? nb : na;                  // the maximum of floats passes over a NaN, which v has too
-    const float ra = na > 0.0f ? 1.0f / na : 0.0f, rb = nb > 0.0f ? __builtin_amdgcn_rsqf(nb) : 0.0f;
-    const float live = nb > 0.0f ? 0x1p127f : 0.0f;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float x = copysignf(__builtin_amdgcn_sqrtf(fabsf(m[j]) * ra), m[j]);
-      const float y = __builtin_amdgcn_sqrtf(r[j] * rb);
-      const float least = __builtin_amdgcn_fmed3f(r[j] * live, 0.0f, 1.0f / 255.0f);   // c >= 1 if v > 0: no
-      m[j] = fmaf(x, 127.0f, kRoundBits);                                              // denominator is lost
-      r[j] = fmaf(fmaxf(y, least), 255.0f, kRoundBits);
-    }
-    *mq = make_uint2(pack_low_bytes(m[0], m[1], m[2], m[3]), pack_low_bytes(m[4], m[5], m[6], m[7]));
-    *vq = make_uint2(pack_low_bytes(r[0], r[1], r[2], r[3]), pack_low_bytes(r[4], r[5], r[6], r[7]));
-    if ((threadIdx.x & 31) == 0) *sc = make_float2(na, nb);
   }
+  const float a1 = c.b1 * ab.x, b2 = c.b2 * ab.y;
+  float ma = 0.0f;
+  unsigned mb = 0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const int qj = (int)((j < 4 ? q.x : q.y) << (24 - 8 * (j & 3))) >> 24;
+    const unsigned wj = ((j < 4 ? w.x : w.y) >> (8 * (j & 3))) & 255u;
+    const float x = (float)qj * (1.0f / 127.0f), y = (float)wj * (1.0f / 255.0f), y2 = y * y;
+    const float gj = g[j] * c.gscale;
+    m[j] = fmaf(a1, x * fabsf(x), c.c1 * gj);
+    const float v = fmaf(b2, y2 * y2, c.c2 * gj * gj);
+    r[j] = __builtin_amdgcn_sqrtf(v);
+    const float u = m[j] * __builtin_amdgcn_rcpf(fmaf(r[j], c.root, c.eps));
+    p[j] -= fmaf(c.decay, p[j], c.size * u);
+    ma = fmaxf(ma, fabsf(m[j]));
+    mb = umax(mb, __float_as_uint(v));      // v is not below zero: its bits order as it does, NaN on top
+  }
+  if (whole) {
+    store<kStream>(P + i, p);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (i + j < end) P[i + j] = from_float<T>(p[j]);
+  }
+  const float nb = block_scale(half_max(mb));
+  float na = block_scale(half_max(__float_as_uint(ma)));
+  na = nb != nb ? nb : na;                  // the maximum of floats passes over a NaN, which v has too
+  const float ra = na > 0.0f ? 1.0f / na : 0.0f, rb = nb > 0.0f ? __builtin_amdgcn_rsqf(nb) : 0.0f;
+  const float live = nb > 0.0f ? 0x1p127f : 0.0f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const float x = copysignf(__builtin_amdgcn_sqrtf(fabsf(m[j]) * ra), m[j]);
+    const float y = __builtin_amdgcn_sqrtf(r[j] * rb);
+    const float least = __builtin_amdgcn_fmed3f(r[j] * live, 0.0f, 1.0f / 255.0f);   // c >= 1 if v > 0: no
+    m[j] = fmaf(x, 127.0f, kRoundBits);                                              // denominator is lost
+    r[j] = fmaf(fmaxf(y, least), 255.0f, kRoundBits);
+  }
+  q = u32x2{pack_low_bytes(m[0], m[1], m[2], m[3]), pack_low_bytes(m[4], m[5], m[6], m[7])};
+  w = u32x2{pack_low_bytes(r[0], r[1], r[2], r[3]), pack_low_bytes(r[4], r[5], r[6], r[7])};
+  if (kStream) {
+    __builtin_nontemporal_store(q, mq);
+    __builtin_nontemporal_store(w, vq);
+  } else {
+    *mq = q;
+    *vq = w;
+  }
+  if ((threadIdx.x & 31) == 0) *sc = make_float2(na, nb);
 }
 
 template <typename T>
 __global__ void __launch_bounds__(kOptThreads)
 moments8_decode_kernel(long n_blocks, const signed char* __restrict__ mq, const unsigned char* __restrict__ vq,
                        const float* __restrict__ scales, T* __restrict__ m, T* __restrict__ v) {
-  const long stride = (long)gridDim.x * kOptThreads * 8;
-  for (long i = 8 * ((long)blockIdx.x * kOptThreads + threadIdx.x); i < n_blocks * kOptBlock; i += stride) {
-    const s8x8 q = *(const s8x8*)(mq + i);
-    const u8x8 w = *(const u8x8*)(vq + i);
-    const float2 ab = ((const float2*)scales)[i / kOptBlock];
-    float x[8], y[8];
+  const long i = 8 * ((long)blockIdx.x * kOptThreads + threadIdx.x);
+  if (i >= n_blocks * kOptBlock) return;
+  const s8x8 q = __builtin_nontemporal_load((const s8x8*)(mq + i));
+  const u8x8 w = __builtin_nontemporal_load((const u8x8*)(vq + i));
+  const float2 ab = ((const float2*)scales)[i / kOptBlock];
+  float x[8], y[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      x[j] = decode_m(q[j], ab.x);
-      y[j] = decode_v(w[j], ab.y);
-    }
-    store(m + i, x);
-    store(v + i, y);
+  for (int j = 0; j < 8; ++j) {
+    x[j] = decode_m(q[j], ab.x);
+    y[j] = decode_v(w[j], ab.y);
   }
+  store<true>(m + i, x);
+  store<true>(v + i, y);
 }
 
 template <typename T>
 __global__ void __launch_bounds__(kOptThreads)
 moments8_encode_kernel(long numel, const T* __restrict__ m, const T* __restrict__ v, signed char* __restrict__ mq,
                        unsigned char* __restrict__ vq, float* __restrict__ scales) {
-  const long stride = (long)gridDim.x * kOptThreads * 8;
-  for (long i = 8 * ((long)blockIdx.x * kOptThreads + threadIdx.x); i - (i & (kOptBlock - 1)) < numel; i += stride) {
-    float x[8], y[8];
-    unsigned ma = 0, mb = 0;
+  const long i = 8 * ((long)blockIdx.x * kOptThreads + threadIdx.x);
+  if (i - (i & (kOptBlock - 1)) >= numel) return;
+  float x[8], y[8];
+  unsigned ma = 0, mb = 0;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      x[j] = i + j < numel ? to_float(m[i + j]) : 0.0f;
-      y[j] = i + j < numel ? to_float(v[i + j]) : 0.0f;
-      ma = umax(ma, magnitude(x[j]));
-      mb = umax(mb, magnitude(y[j]));
-    }
-    const float a = block_scale(half_max(ma)), b = block_scale(half_max(mb));
-    s8x8 q;
-    u8x8 w;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      q[j] = (signed char)encode_m(x[j], a);
-      w[j] = (unsigned char)encode_v(y[j], b);
-    }
-    *(s8x8*)(mq + i) = q;
-    *(u8x8*)(vq + i) = w;
-    if ((threadIdx.x & 31) == 0) ((float2*)scales)[i / kOptBlock] = make_float2(a, b);
+  for (int j = 0; j < 8; ++j) {
+    x[j] = i + j < numel ? to_float(m[i + j]) : 0.0f;
+    y[j] = i + j < numel ? to_float(v[i + j]) : 0.0f;
+    ma = umax(ma, magnitude(x[j]));
+    mb = umax(mb, magnitude(y[j]));
   }
+  const float a = block_scale(half_max(ma)), b = block_scale(half_max(mb));
+  s8x8 q;
+  u8x8 w;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    q[j] = (signed char)encode_m(x[j], a);
+    w[j] = (unsigned char)encode_v(y[j], b);
+  }
+  *(s8x8*)(mq + i) = q;
+  *(u8x8*)(vq + i) = w;
+  if ((threadIdx.x & 31) == 0) ((float2*)scales)[i / kOptBlock] = make_float2(a, b);
 }
 
 // ---- norms: squares and sums in 64 bits (no overflow for any fp32 gradient), one partial sum per workgroup, added up
@@ -404,16 +400,16 @@ __device__ inline double wave_sum(double x) {
 }
 
 // 16 bytes a thread and load, four of them in flight
-template <typename T>
+template <bool kStream, typename T>
 __device__ inline double sum_squares(const T* __restrict__ g, long base, long end) {
   constexpr int N = 16 / sizeof(T);
-  constexpr long kRow = (long)N * kOptThreads;
+  constexpr long kRow = (long)N * kNormThreads;
   double s0 = 0.0, s1 = 0.0;
   long i = base + N * threadIdx.x;
   for (; i + 3 * kRow + N <= end; i += 4 * kRow) {
     float x[4][N];
 #pragma unroll
-    for (int h = 0; h < 4; ++h) load(x[h], g + i + h * kRow);
+    for (int h = 0; h < 4; ++h) load<kStream>(x[h], g + i + h * kRow);
 #pragma unroll
     for (int h = 0; h < 4; ++h)
 #pragma unroll
@@ -425,7 +421,7 @@ __device__ inline double sum_squares(const T* __restrict__ g, long base, long en
   for (; i < end; i += kRow) {
     float x[N];
     if (i + N <= end) {
-      load(x, g + i);
+      load<kStream>(x, g + i);
     } else {
 #pragma unroll
       for (int j = 0; j < N; ++j) x[j] = i + j < end ? to_float(g[i + j]) : 0.0f;
@@ -439,21 +435,24 @@ __device__ inline double sum_squares(const T* __restrict__ g, long base, long en
   return s0 + s1;
 }
 
-__global__ void __launch_bounds__(kOptThreads)
+template <bool kStream>
+__global__ void __launch_bounds__(kNormThreads)
 norm_partial_kernel(const NormTable tab) {
-  __shared__ double part[kOptThreads / 64];
+  __shared__ double part[kNormThreads / 64];
   const int k = find_tensor(tab.first, tab.n, blockIdx.x);
   const long base = (long)(blockIdx.x - tab.first[k]) * tab.chunk, numel = tab.numel[k] >> 2;
   const long end = base + tab.chunk < numel ? base + tab.chunk : numel;
   const int dtype = tab.numel[k] & 3;
   double s;
-  if (dtype == PIR_F32) s = sum_squares((const float*)tab.grad[k], base, end);
-  else if (dtype == PIR_BF16) s = sum_squares((const __bf16*)tab.grad[k], base, end);
-  else s = sum_squares((const _Float16*)tab.grad[k], base, end);
+  if (dtype == PIR_F32) s = sum_squares<kStream>((const float*)tab.grad[k], base, end);
+  else if (dtype == PIR_BF16) s = sum_squares<kStream>((const __bf16*)tab.grad[k], base, end);
+  else s = sum_squares<kStream>((const _Float16*)tab.grad[k], base, end);
   s = wave_sum(s);
   if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = s;
   __syncthreads();
-  if (threadIdx.x == 0) tab.partial[blockIdx.x] = part[0] + part[1] + part[2] + part[3];
+  if (threadIdx.x != 0) return;
+  for (int w = 1; w < kNormThreads / 64; ++w) s += part[w];
+  tab.partial[blockIdx.x] = s;
 }
 
 // sum of the partials by a workgroup of kPrepThreads
@@ -544,20 +543,24 @@ norm_finish_kernel(int n, const unsigned* __restrict__ first, int n_partial, con
 
 static inline long ceil_div(long a, long b) { return (a + b - 1) / b; }
 
-static const long kMaxGroups = (1L << 24) - 1;     // workgroups of 256 threads: a grid has fewer than 2^32 threads
-static const long kMaxNumel = 1L << 34;            // of a tensor: what kMaxGroups of the smallest chunk reach
-static const long kMaxTotal = 1L << 36;            // of a call
+static const long kMaxGroups = (1L << 24) - 1;     // workgroups: a grid has fewer than 2^32 threads
+static const long kCacheBytes = 256L << 20;        // last-level cache
 
-static int check_tensors(int n, const long* numels, const int* dtypes, const void* const* grads) {
+// scales[i]: whether tensor i has 8-bit moments (scales NULL: none has)
+static int check_tensors(int n, const long* numels, const int* dtypes, const void* const* grads, float* const* scales) {
   if (n < 0 || (n > 0 && (!numels || !dtypes || !grads))) return PIR_ERR_ARG;
-  long total = 0;
+  long groups = 0;
   for (int i = 0; i < n; ++i) {
     if (numels[i] < 0 || dtypes[i] < PIR_F32 || dtypes[i] > PIR_F16) return PIR_ERR_ARG;
     if (numels[i] > 0 && !grads[i]) return PIR_ERR_ARG;
-    if (numels[i] > kMaxNumel || (total += numels[i]) > kMaxTotal) return PIR_ERR_TOO_LARGE;
+    if (numels[i] > kMaxGroups * kOptChunk8) return PIR_ERR_TOO_LARGE;
+    groups += ceil_div(numels[i], scales && scales[i] ? kOptChunk8 : kOptChunk);
+    if (groups > kMaxGroups) return PIR_ERR_TOO_LARGE;
   }
   return PIR_OK;
 }
+
+static inline long element_bytes(int dtype) { return dtype == PIR_F32 ? 4 : 2; }
 
 // Elements a workgroup takes: as few as fill the card when there is little to do, more of them when there is much, so
 // that the search for its tensor and the second pass over the partial sums stay small beside it.
@@ -582,11 +585,14 @@ static int launch_partials(int n, const void* const* grads, const long* numels, 
   tab.n = 0;
   tab.chunk = norm_chunk(n, numels);
   tab.partial = partial;
-  long at = 0;                                  // workgroups of this launch so far
+  long at = 0, bytes = 0;                       // workgroups of this launch so far
+  for (int i = 0; i < n; ++i) bytes += numels[i] * element_bytes(dtypes[i]);
   for (int i = 0; i <= n; ++i) {
     const long blocks = i < n ? ceil_div(numels[i], tab.chunk) : 0;
-    if (tab.n > 0 && (i == n || tab.n == kNormTable || at + blocks > kMaxGroups)) {
-      hipLaunchKernelGGL(norm_partial_kernel, dim3((unsigned)at), dim3(kOptThreads), 0, stream, tab);
+    if (tab.n > 0 && (i == n || tab.n == kNormTable)) {
+      const dim3 grid((unsigned)at), block(kNormThreads);
+      if (bytes > kCacheBytes) hipLaunchKernelGGL(norm_partial_kernel<true>, grid, block, 0, stream, tab);
+      else hipLaunchKernelGGL(norm_partial_kernel<false>, grid, block, 0, stream, tab);
       tab.partial += at;
       tab.n = 0;
       at = 0;
@@ -601,15 +607,16 @@ static int launch_partials(int n, const void* const* grads, const long* numels, 
   return pir_check_launch();
 }
 
+template <bool kStream>
 static void launch_update(int kind, const UpdateArgs& args, long groups, hipStream_t stream) {
   const dim3 grid((unsigned)groups), block(kOptThreads);
   switch (kind) {
-    case PIR_F32: hipLaunchKernelGGL(adamw32_kernel<float>, grid, block, 0, stream, args); break;
-    case PIR_BF16: hipLaunchKernelGGL(adamw32_kernel<__bf16>, grid, block, 0, stream, args); break;
-    case PIR_F16: hipLaunchKernelGGL(adamw32_kernel<_Float16>, grid, block, 0, stream, args); break;
-    case 3 + PIR_F32: hipLaunchKernelGGL(adamw8_kernel<float>, grid, block, 0, stream, args); break;
-    case 3 + PIR_BF16: hipLaunchKernelGGL(adamw8_kernel<__bf16>, grid, block, 0, stream, args); break;
-    default: hipLaunchKernelGGL(adamw8_kernel<_Float16>, grid, block, 0, stream, args);
+    case PIR_F32: hipLaunchKernelGGL((adamw32_kernel<float, kStream>), grid, block, 0, stream, args); break;
+    case PIR_BF16: hipLaunchKernelGGL((adamw32_kernel<__bf16, kStream>), grid, block, 0, stream, args); break;
+    case PIR_F16: hipLaunchKernelGGL((adamw32_kernel<_Float16, kStream>), grid, block, 0, stream, args); break;
+    case 3 + PIR_F32: hipLaunchKernelGGL((adamw8_kernel<float, kStream>), grid, block, 0, stream, args); break;
+    case 3 + PIR_BF16: hipLaunchKernelGGL((adamw8_kernel<__bf16, kStream>), grid, block, 0, stream, args); break;
+    default: hipLaunchKernelGGL((adamw8_kernel<_Float16, kStream>), grid, block, 0, stream, args);
   }
 }
 
@@ -643,7 +650,7 @@ int pir_adamw_step(int n, void* const* params, const void* const* grads, void* c
                    const PirAdamwGroup* group, int n_groups, double max_norm, int skip_nonfinite, float* total_norm,
                    void* workspace, size_t workspace_bytes, void* stream_) {
   hipStream_t stream = (hipStream_t)stream_;
-  const int rc = check_tensors(n, numels, dtypes, grads);
+  const int rc = check_tensors(n, numels, dtypes, grads, scales);
   if (rc != PIR_OK) return rc;
   if (n > 0 && (!params || !exp_avgs || !exp_avg_sqs || !steps || !groups || !group || n_groups < 1)) return PIR_ERR_ARG;
   for (int k = 0; k < n_groups && n > 0; ++k) {
@@ -666,10 +673,8 @@ int pir_adamw_step(int n, void* const* params, const void* const* grads, void* c
   OptCoef* coef = (OptCoef*)(ws + space.coef);
   unsigned* first = (unsigned*)(ws + space.first);
   double* partial = (double*)(ws + space.partial);
-  long total = 0;
-  for (int i = 0; i < n; ++i) total += numels[i];
-  const unsigned chunk = total > (16L << 20) ? 8192 : 2048;
-  if (total / chunk + n > kMaxGroups) return PIR_ERR_TOO_LARGE;
+  long bytes = 0;                               // what the update touches: parameter, gradient, two moments
+  for (int i = 0; i < n; ++i) bytes += numels[i] * (2 * element_bytes(dtypes[i]) + (scales && scales[i] ? 2 : 8));
   if (with_norm && launch_partials(n, grads, numels, dtypes, partial, stream) != PIR_OK) return PIR_ERR_LAUNCH;
 
   PrepTable tab;
@@ -730,15 +735,16 @@ int pir_adamw_step(int n, void* const* params, const void* const* grads, void* c
       r.step = steps[i];
       r.first = (unsigned)kinds[kind].groups;
       r.group = (unsigned)j;
-      kinds[kind].groups += ceil_div(numels[i], chunk);
+      kinds[kind].groups += ceil_div(numels[i], kind >= 3 ? kOptChunk8 : kOptChunk);
       ++kinds[kind].n;
     }
   }
   if (tab.n > 0 || tab.finalize) prologue();
   int row = 0;
   for (int kind = 0; kind < 6; ++kind) {
-    const UpdateArgs args = {rows + row, coef + row, first + row, kinds[kind].n, chunk};
-    if (kinds[kind].groups > 0) launch_update(kind, args, kinds[kind].groups, stream);
+    const UpdateArgs args = {rows + row, coef + row, first + row, kinds[kind].n};
+    if (kinds[kind].groups > 0 && bytes > kCacheBytes) launch_update<true>(kind, args, kinds[kind].groups, stream);
+    else if (kinds[kind].groups > 0) launch_update<false>(kind, args, kinds[kind].groups, stream);
     row += kinds[kind].n;
   }
   return pir_check_launch();
@@ -752,7 +758,7 @@ size_t pir_grad_norm_workspace_bytes(int n, const long* numels) {
 int pir_grad_norm(int n, const void* const* grads, const long* numels, const int* dtypes, float* total, float* each,
                   void* workspace, size_t workspace_bytes, void* stream_) {
   hipStream_t stream = (hipStream_t)stream_;
-  const int rc = check_tensors(n, numels, dtypes, grads);
+  const int rc = check_tensors(n, numels, dtypes, grads, nullptr);
   if (rc != PIR_OK) return rc;
   if (!total) return PIR_ERR_ARG;
   if (!workspace || workspace_bytes < pir_grad_norm_workspace_bytes(n, numels)) return PIR_ERR_SCRATCH;
@@ -780,18 +786,14 @@ int pir_grad_norm(int n, const void* const* grads, const long* numels, const int
   return pir_check_launch();
 }
 
-static unsigned moments8_grid(long n_blocks) {
-  const long g = ceil_div(n_blocks, 8), cap = 32L * pir_num_cus();
-  return (unsigned)(g < cap ? g : cap);
-}
-
 int pir_moments8_decode(long n_blocks, const signed char* exp_avg, const unsigned char* exp_avg_sq, const float* scales,
                         int dtype, void* m, void* v, void* stream) {
   if (n_blocks < 0 || dtype < PIR_F32 || dtype > PIR_F16) return PIR_ERR_ARG;
+  if (n_blocks > kMaxGroups * (kOptChunk8 / kOptBlock)) return PIR_ERR_TOO_LARGE;
   if (n_blocks == 0) return PIR_OK;
   if (!exp_avg || !exp_avg_sq || !scales || !m || !v || ((((size_t)exp_avg | (size_t)exp_avg_sq) & 15) || ((size_t)scales & 7)))
     return PIR_ERR_ARG;
-  const dim3 grid(moments8_grid(n_blocks)), block(kOptThreads);
+  const dim3 grid((unsigned)ceil_div(n_blocks * kOptBlock, kOptChunk8)), block(kOptThreads);
   hipStream_t s = (hipStream_t)stream;
   if (dtype == PIR_F32)
     hipLaunchKernelGGL(moments8_decode_kernel<float>, grid, block, 0, s, n_blocks, exp_avg, exp_avg_sq, scales, (float*)m, (float*)v);
@@ -805,11 +807,11 @@ int pir_moments8_decode(long n_blocks, const signed char* exp_avg, const unsigne
 int pir_moments8_encode(long numel, int dtype, const void* m, const void* v, signed char* exp_avg,
                         unsigned char* exp_avg_sq, float* scales, void* stream) {
   if (numel < 0 || dtype < PIR_F32 || dtype > PIR_F16) return PIR_ERR_ARG;
+  if (numel > kMaxGroups * kOptChunk8) return PIR_ERR_TOO_LARGE;
   if (numel == 0) return PIR_OK;
   if (!exp_avg || !exp_avg_sq || !scales || !m || !v || ((((size_t)exp_avg | (size_t)exp_avg_sq) & 15) || ((size_t)scales & 7)))
     return PIR_ERR_ARG;
-  const long n_blocks = ceil_div(numel, kOptBlock);
-  const dim3 grid(moments8_grid(n_blocks)), block(kOptThreads);
+  const dim3 grid((unsigned)ceil_div(numel, kOptChunk8)), block(kOptThreads);
   hipStream_t s = (hipStream_t)stream;
   if (dtype == PIR_F32)
     hipLaunchKernelGGL(moments8_encode_kernel<float>, grid, block, 0, s, numel, (const float*)m, (const float*)v, exp_avg, exp_avg_sq, scales);
