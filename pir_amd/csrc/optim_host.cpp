@@ -17,6 +17,7 @@ using StepFn = decltype(&pir_adamw_step);
 using StepBytesFn = decltype(&pir_adamw_workspace_bytes);
 using NormFn = decltype(&pir_grad_norm);
 using NormBytesFn = decltype(&pir_grad_norm_workspace_bytes);
+using DecodeFn = decltype(&pir_moments8_decode);
 
 // borrowed items of a list
 struct Items {
@@ -31,7 +32,7 @@ struct Items {
 
 // a plain dense tensor of this device, or null
 const at::Tensor* tensor_of(PyObject* o, c10::Device dev) {
-  if (!THPVariable_Check(o)) return nullptr;
+  if (!PyType_IsSubtype(Py_TYPE(o), (PyTypeObject*)THPVariableClass)) return nullptr;
   const at::Tensor& t = THPVariable_Unpack(o);
   if (!t.defined() || t.layout() != at::kStrided || t.device() != dev || t.is_neg() ||
       t.unsafeGetTensorImpl()->is_python_dispatch())
@@ -56,6 +57,14 @@ bool same_layout(const at::Tensor& p, const at::Tensor& t) {
 bool dense(const at::Tensor& t) { return t.is_contiguous() || t.is_non_overlapping_and_dense(); }
 
 char* address(const at::Tensor& t) { return (char*)t.unsafeGetTensorImpl()->mutable_data(); }
+
+// whether these are the 8-bit moments of nb blocks as the kernels read them
+bool coded(const at::Tensor& q, const at::Tensor& c, const at::Tensor& s, long nb) {
+  return q.scalar_type() == at::kChar && c.scalar_type() == at::kByte && s.scalar_type() == at::kFloat && q.is_contiguous() &&
+         c.is_contiguous() && s.is_contiguous() && q.dim() == 2 && q.size(0) == nb && q.size(1) == 256 && c.sizes() == q.sizes() &&
+         s.dim() == 2 && s.size(0) == nb && s.size(1) == 2 && !(((size_t)address(q) | (size_t)address(c)) & 15) &&
+         !((size_t)address(s) & 7);
+}
 
 // whether no byte belongs to two of the tensors; most lists are in the order of memory already
 bool disjoint(const std::vector<void*>& at, const std::vector<long>& bytes, std::vector<std::pair<char*, long>>& scratch) {
@@ -87,15 +96,16 @@ PyObject* fail(const char* what, int code) {
   return PyErr_Format(PyExc_RuntimeError, "%s failed (code %d)", what, code);
 }
 
-// adamw_step(fn, bytes_fn, params, grads, exp_avgs, exp_avg_sqs, scales | None, steps: tensor or list, groups: array of
-// int | None, group table, n_groups, max_norm, skip_nonfinite, want_norm, device index, stream) -> norm | None
+// adamw_step(fn, bytes_fn, params, grads, exp_avgs, exp_avg_sqs, scales | None, steps: tensor or list, groups: address of
+// an int for each tensor | 0, list of (lr, beta1, beta2, eps, weight decay, address of the lr on the device | 0),
+// max_norm, skip_nonfinite, want_norm, device index, stream) -> norm | None
 PyObject* step(PyObject*, PyObject* args) {
-  unsigned long long fn, bytes_fn, groups_at, table, stream;
-  PyObject *params, *grads, *ms, *vs, *ss, *ts;
-  int n_groups, skip, want, index;
+  unsigned long long fn, bytes_fn, groups_at, stream;
+  PyObject *params, *grads, *ms, *vs, *ss, *ts, *hypers;
+  int skip, want, index;
   double max_norm;
-  if (!PyArg_ParseTuple(args, "KKOOOOOOKKidppiK", &fn, &bytes_fn, &params, &grads, &ms, &vs, &ss, &ts, &groups_at, &table,
-                        &n_groups, &max_norm, &skip, &want, &index, &stream))
+  if (!PyArg_ParseTuple(args, "KKOOOOOOKO!dppiK", &fn, &bytes_fn, &params, &grads, &ms, &vs, &ss, &ts, &groups_at,
+                        &PyList_Type, &hypers, &max_norm, &skip, &want, &index, &stream))
     return nullptr;
   try {
     const c10::Device dev(c10::kCUDA, (c10::DeviceIndex)index);
@@ -122,12 +132,8 @@ PyObject* step(PyObject*, PyObject* args) {
       } else {
         const at::Tensor* s = tensor_of(so, dev);
         const long nb = (numel + 255) / 256;
-        if (!s || s->scalar_type() != at::kFloat || m->scalar_type() != at::kChar || v->scalar_type() != at::kByte ||
-            !m->is_contiguous() || !v->is_contiguous() || !s->is_contiguous() || m->dim() != 2 || m->size(0) != nb ||
-            m->size(1) != 256 || v->sizes() != m->sizes() || s->dim() != 2 || s->size(0) != nb || s->size(1) != 2)
-          Py_RETURN_NOTIMPLEMENTED;
+        if (!s || !coded(*m, *v, *s, nb)) Py_RETURN_NOTIMPLEMENTED;
         as = address(*s);
-        if ((((size_t)am | (size_t)av) & 15) || ((size_t)as & 7)) Py_RETURN_NOTIMPLEMENTED;
         if (!as) as = (char*)16;                 // no blocks: 8-bit all the same
         a.mbytes[i] = a.vbytes[i] = 256 * nb;
       }
@@ -155,6 +161,14 @@ PyObject* step(PyObject*, PyObject* args) {
     std::vector<std::pair<char*, long>> scratch;
     if (!disjoint(a.p, a.bytes, scratch) || !disjoint(a.m, a.mbytes, scratch) || !disjoint(a.v, a.vbytes, scratch))
       Py_RETURN_NOTIMPLEMENTED;
+    std::vector<PirAdamwGroup> table(PyList_GET_SIZE(hypers));
+    for (size_t k = 0; k < table.size(); ++k) {
+      unsigned long long lr = 0;
+      PirAdamwGroup& h = table[k];
+      if (!PyArg_ParseTuple(PyList_GET_ITEM(hypers, k), "dddddK", &h.lr, &h.beta1, &h.beta2, &h.eps, &h.weight_decay, &lr))
+        return nullptr;
+      h.lr_device = (const float*)lr;
+    }
     std::vector<int> zeros;
     if (!groups_at) zeros.resize(n, 0);
     const int with_norm = want || skip || max_norm > 0.0;
@@ -166,7 +180,7 @@ PyObject* step(PyObject*, PyObject* args) {
     const int code = ((StepFn)fn)((int)n, a.p.data(), (const void* const*)a.g.data(), a.m.data(), a.v.data(),
                                   ss == Py_None ? nullptr : (float* const*)a.s.data(), (float* const*)a.t.data(),
                                   a.numels.data(), a.dtypes.data(), groups_at ? (const int*)groups_at : zeros.data(),
-                                  (const PirAdamwGroup*)table, n_groups, max_norm, skip,
+                                  table.data(), (int)table.size(), max_norm, skip,
                                   with_norm ? norm.data_ptr<float>() : nullptr, work.data_ptr(), size, (void*)stream);
     if (code != PIR_OK) return fail("pir_adamw_step", code);
     for (Py_ssize_t i = 0; i < n; ++i) {         // autograd and the networks' packed weights go by the version
@@ -215,7 +229,37 @@ PyObject* norm(PyObject*, PyObject* args) {
   }
 }
 
-PyMethodDef methods[] = {{"adamw_step", step, METH_VARARGS, nullptr}, {"grad_norm", norm, METH_VARARGS, nullptr}, {nullptr, nullptr, 0, nullptr}};
+// moments8_decode(fn, exp_avg, exp_avg_sq, scales, type, device index, stream) -> (m, v)
+PyObject* decode(PyObject*, PyObject* args) {
+  unsigned long long fn, stream;
+  PyObject *qo, *co, *so;
+  int type, index;
+  if (!PyArg_ParseTuple(args, "KOOOiiK", &fn, &qo, &co, &so, &type, &index, &stream)) return nullptr;
+  try {
+    const c10::Device dev(c10::kCUDA, (c10::DeviceIndex)index);
+    const at::Tensor *q = tensor_of(qo, dev), *c = tensor_of(co, dev), *s = tensor_of(so, dev);
+    if (!q || !c || !s || !coded(*q, *c, *s, q->dim() ? q->size(0) : 0)) Py_RETURN_NOTIMPLEMENTED;
+    const c10::OptionalDeviceGuard guard(dev);
+    const auto as = at::TensorOptions().dtype(type == PIR_F32 ? at::kFloat : type == PIR_BF16 ? at::kBFloat16 : at::kHalf).device(dev);
+    const at::Tensor m = at::empty(q->sizes(), as), v = at::empty(q->sizes(), as);
+    const int code = ((DecodeFn)fn)(q->size(0), (const signed char*)address(*q), (const unsigned char*)address(*c),
+                                    (const float*)address(*s), type, m.data_ptr(), v.data_ptr(), (void*)stream);
+    if (code != PIR_OK) return fail("pir_moments8_decode", code);
+    PyObject* pair = PyTuple_New(2);
+    if (!pair) return nullptr;
+    PyTuple_SET_ITEM(pair, 0, THPVariable_Wrap(m));
+    PyTuple_SET_ITEM(pair, 1, THPVariable_Wrap(v));
+    return pair;
+  } catch (const std::exception& e) {
+    PyErr_SetString(PyExc_RuntimeError, e.what());
+    return nullptr;
+  }
+}
+
+PyMethodDef methods[] = {{"adamw_step", step, METH_VARARGS, nullptr},
+                         {"grad_norm", norm, METH_VARARGS, nullptr},
+                         {"moments8_decode", decode, METH_VARARGS, nullptr},
+                         {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_optim_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -37,28 +37,24 @@ _TINY = 2.0 ** -126              # blocks whose largest is below this are zero
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
-class _Group(ctypes.Structure):
-    _fields_ = [(k, ctypes.c_double) for k in ("lr", "beta1", "beta2", "eps", "weight_decay")] + [("lr_device", ctypes.c_void_p)]
-
-
 def _hyper(lr, betas, eps, weight_decay, device):
-    """Checked hyper-parameters of one group; a learning rate on the device stays there."""
-    dev_lr = None
+    """Checked hyper-parameters of one group, and the address of a learning rate that stays on the device, or 0."""
+    dev_lr = 0
     if isinstance(lr, torch.Tensor):
         if lr.numel() != 1:
             raise ValueError("lr: a number or a tensor of one element")
         if lr.is_cuda:
             if lr.dtype != torch.float32 or lr.device != device:
                 raise ValueError("lr: a device tensor has to be float32, on the device of the parameters")
-            dev_lr, lr = lr, 0.0
-    lr, beta1, beta2 = float(lr), float(betas[0]), float(betas[1])
+            dev_lr, lr = lr.data_ptr(), 0.0
+    lr, beta1, beta2, eps, weight_decay = float(lr), float(betas[0]), float(betas[1]), float(eps), float(weight_decay)
     if not 0.0 <= lr < math.inf:
         raise ValueError(f"lr out of range: {lr}")
     if not (0.0 <= beta1 < 1.0 and 0.0 <= beta2 < 1.0):
         raise ValueError(f"betas out of range: {betas}")
-    if not (0.0 <= float(eps) < math.inf and 0.0 <= float(weight_decay) < math.inf):
+    if not (0.0 <= eps < math.inf and 0.0 <= weight_decay < math.inf):
         raise ValueError(f"eps or weight_decay out of range: {eps}, {weight_decay}")
-    return dev_lr, lr, beta1, beta2, float(eps), float(weight_decay)
+    return lr, beta1, beta2, eps, weight_decay, dev_lr
 
 
 def _max_norm(max_norm):
@@ -158,22 +154,23 @@ def _host():
             from . import _optim_host
         except ImportError as e:
             raise _lib.PirHipError(f"pir_amd/_optim_host.so: {e}; build it first (python -m pir_amd.build)") from e
-        names = ("pir_adamw_step", "pir_adamw_workspace_bytes", "pir_grad_norm", "pir_grad_norm_workspace_bytes")
+        names = ("pir_adamw_step", "pir_adamw_workspace_bytes", "pir_grad_norm", "pir_grad_norm_workspace_bytes",
+                 "pir_moments8_decode")
         _native = (_optim_host, *(ctypes.cast(getattr(L, n), ctypes.c_void_p).value for n in names))
     return _native
+
+
+def _stream(dev):
+    return torch._C._cuda_getCurrentRawStream(dev.index)
 
 
 def _run(params, grads, exp_avgs, exp_avg_sqs, scales, steps, groups, hypers, max_norm, skip_nonfinite, want_norm):
     """One pir_adamw_step.  steps: a tensor with one count per parameter, or a list of them; groups: index into hypers of
     each tensor, an array of int (None: all in the first)."""
     dev = params[0].device
-    table = (_Group * len(hypers))()
-    for row, (dev_lr, lr, beta1, beta2, eps, decay) in zip(table, hypers):
-        row.lr, row.beta1, row.beta2, row.eps, row.weight_decay = lr, beta1, beta2, eps, decay
-        row.lr_device = None if dev_lr is None else dev_lr.data_ptr()
-    host, step, size, _, _ = _host()
-    rest = (exp_avgs, exp_avg_sqs, scales, steps, 0 if groups is None else groups.buffer_info()[0], ctypes.addressof(table),
-            len(hypers), max_norm, skip_nonfinite, want_norm, dev.index, torch.cuda.current_stream(dev).cuda_stream)
+    host, step, size, *_ = _host()
+    rest = (exp_avgs, exp_avg_sqs, scales, steps, 0 if groups is None else groups.buffer_info()[0], hypers, max_norm,
+            skip_nonfinite, want_norm, dev.index, _stream(dev))
     norm = host.adamw_step(step, size, params, grads, *rest)
     if norm is NotImplemented:
         grads = _check(params, grads, exp_avgs, exp_avg_sqs, scales)
@@ -195,7 +192,7 @@ def _run_torch(params, grads, exp_avgs, exp_avg_sqs, scales, steps, groups, hype
             if skip_nonfinite and not torch.isfinite(norm):
                 return norm
         for i, (p, g, m, v, t) in enumerate(zip(params, grads, exp_avgs, exp_avg_sqs, steps)):
-            _, lr, beta1, beta2, eps, decay = hypers[groups[i]]
+            lr, beta1, beta2, eps, decay, _ = hypers[groups[i]]
             t.add_(1)
             count = float(t)
             s = scales[i] if scales is not None else None
@@ -229,7 +226,7 @@ def _step(params, grads, exp_avgs, exp_avg_sqs, scales, steps, lr, betas, eps, w
         return torch.zeros((), device=dev) if want or skip_nonfinite else None
     if params[0].device != dev:
         raise ValueError("steps: on another device than the parameters")
-    if hyper[0] is not None and not dev.type == "cuda":
+    if hyper[5] and dev.type != "cuda":
         raise ValueError("lr: on another device than the parameters")
     if dev.type != "cuda":
         grads = _check(params, grads, exp_avgs, exp_avg_sqs, scales)
@@ -272,13 +269,12 @@ def grad_norm(tensors):
             _check_norm(tensors, dev)
             each = torch.stack([t.double().square().sum() for t in tensors])
             return each.sum().sqrt().float(), each.sqrt().float()
-        host, _, _, norm, size = _host()
-        stream = torch.cuda.current_stream(dev).cuda_stream
-        out = host.grad_norm(norm, size, tensors, dev.index, stream)
+        host, _, _, norm, size, _ = _host()
+        out = host.grad_norm(norm, size, tensors, dev.index, _stream(dev))
         if out is NotImplemented:
             _check_norm(tensors, dev)
             tensors = [t.resolve_neg() if _dense(t) else t.contiguous() for t in tensors]
-            out = host.grad_norm(norm, size, tensors, dev.index, stream)
+            out = host.grad_norm(norm, size, tensors, dev.index, _stream(dev))
             if out is NotImplemented:
                 raise ValueError("plain tensors of one device are wanted")
     return out[0], out[1:]
@@ -319,8 +315,7 @@ def moments8_encode(exp_avg, exp_avg_sq):
                torch.empty(nb, 2, dtype=torch.float32, device=dev))
         with torch.cuda.device(dev):
             _lib.check(_lib.lib().pir_moments8_encode(numel, _DTYPES[m.dtype], m.data_ptr(), v.data_ptr(),
-                                                      *[t.data_ptr() for t in out],
-                                                      torch.cuda.current_stream(dev).cuda_stream), "pir_moments8_encode")
+                                                      *[t.data_ptr() for t in out], _stream(dev)), "pir_moments8_encode")
         return out
 
 
@@ -329,20 +324,18 @@ def moments8_decode(exp_avg, exp_avg_sq, scales, dtype=torch.float32):
     q, c, s = exp_avg, exp_avg_sq, scales
     if dtype not in _DTYPES:
         raise ValueError(f"dtype: {dtype} is not supported (float32, bfloat16, float16)")
+    if q.is_cuda:
+        host, *_, decode = _host()
+        out = host.moments8_decode(decode, q, c, s, _DTYPES[dtype], q.device.index, _stream(q.device))
+        if out is not NotImplemented:
+            return out
     if q.dtype != torch.int8 or c.dtype != torch.uint8 or s.dtype != torch.float32 or q.dim() != 2 or q.shape[1] != BLOCK \
             or c.shape != q.shape or tuple(s.shape) != (q.shape[0], 2) or not (q.device == c.device == s.device) \
             or not (q.is_contiguous() and c.is_contiguous() and s.is_contiguous()):
         raise ValueError("moments: contiguous int8 and uint8 [blocks, 256] with float32 scales [blocks, 2] are wanted")
-    if q.device.type != "cuda":
-        return tuple(x.to(dtype) for x in _decode_torch(q, c, s))
-    if (q.data_ptr() | c.data_ptr()) % 16 or s.data_ptr() % 8:
+    if q.is_cuda:
         raise ValueError("moments: codes have to start at a multiple of 16 bytes, scales of 8")
-    m, v = (torch.empty(q.shape, dtype=dtype, device=q.device) for _ in range(2))
-    with torch.cuda.device(q.device):
-        _lib.check(_lib.lib().pir_moments8_decode(q.shape[0], q.data_ptr(), c.data_ptr(), s.data_ptr(), _DTYPES[dtype],
-                                                  m.data_ptr(), v.data_ptr(),
-                                                  torch.cuda.current_stream(q.device).cuda_stream), "pir_moments8_decode")
-    return m, v
+    return tuple(x.to(dtype) for x in _decode_torch(q, c, s))
 
 
 # ------------------------------------------------------------------------------------------------- the optimizer
@@ -463,7 +456,7 @@ def step_together(optimizers, max_norm=None, skip_nonfinite=False):
     norm = torch.zeros(()) if max_norm is not None or skip_nonfinite else None      # what no gradients have
     for dev, (params, index, owners) in by_device.items():
         hypers = [_hyper(g["lr"], g["betas"], g["eps"], g["weight_decay"], dev) for _, g in owners]
-        if dev.type != "cuda" and any(h[0] is not None for h in hypers):
+        if dev.type != "cuda" and any(h[5] for h in hypers):
             raise ValueError("lr: on another device than the parameters")
         states = [owners[k][0]._state_of(p, owners[k][1]) for p, k in zip(params, index)]
         m, v, t = ([s[k] for s in states] for k in ("exp_avg", "exp_avg_sq", "step"))

@@ -318,12 +318,16 @@ def test_training_steps_with_adamw(monkeypatch):
 
 
 # ---- the C entry points' host checks: every call here is refused before anything is launched
+class Group(ctypes.Structure):
+    _fields_ = [(k, ctypes.c_double) for k in ("lr", "beta1", "beta2", "eps", "weight_decay")] + [("lr_device", ctypes.c_void_p)]
+
+
 def c_step(n=1, **change):
     from pir_amd import _lib
     L = _lib.lib()
     one = (ctypes.c_void_p * 4)(*[4096] * 4)             # never read: the checks come first
     args = dict(params=one, grads=one, m=one, v=one, scales=None, steps=one, numels=(ctypes.c_long * 4)(*[10] * 4),
-                dtypes=(ctypes.c_int * 4)(), groups=(ctypes.c_int * 4)(), group=(optim._Group * 1)(optim._Group(1e-3, 0.9, 0.99, 1e-8, 0.0, None)),
+                dtypes=(ctypes.c_int * 4)(), groups=(ctypes.c_int * 4)(), group=(Group * 1)(Group(1e-3, 0.9, 0.99, 1e-8, 0.0, None)),
                 n_groups=1, max_norm=0.0, skip=0, norm=None, work=4096, size=0, stream=None)
     args.update(change)
     at = lambda x: ctypes.addressof(x) if isinstance(x, ctypes.Array) else x  # noqa: E731
@@ -337,8 +341,8 @@ def c_step(n=1, **change):
     (1, dict(grads=(ctypes.c_void_p * 1)(None))), (1, dict(params=(ctypes.c_void_p * 1)(None))), (1, dict(steps=(ctypes.c_void_p * 1)(None))),
     (1, dict(scales=(ctypes.c_void_p * 1)(4), m=(ctypes.c_void_p * 1)(4096))),
     (1, dict(scales=(ctypes.c_void_p * 1)(4096), m=(ctypes.c_void_p * 1)(4100))),
-    (1, dict(group=(optim._Group * 1)(optim._Group(1e-3, 1.0, 0.99, 1e-8, 0.0, None)))),
-    (1, dict(group=(optim._Group * 1)(optim._Group(math.nan, 0.9, 0.99, 1e-8, 0.0, None)))),
+    (1, dict(group=(Group * 1)(Group(1e-3, 1.0, 0.99, 1e-8, 0.0, None)))),
+    (1, dict(group=(Group * 1)(Group(math.nan, 0.9, 0.99, 1e-8, 0.0, None)))),
     (3, dict(size=16)), (3, dict(work=None, size=1 << 20)),
     (4, dict(numels=(ctypes.c_long * 1)(1 << 60))),
 ])
