@@ -19,13 +19,13 @@ constexpr int kOptThreads = 256;
 constexpr int kOptBlock = 256;                // elements that share a scale
 constexpr int kOptChunk = 1024;               // elements one workgroup updates, with 32-bit moments
 constexpr int kOptChunk8 = 2048;              // and with 8-bit ones
-constexpr int kPrepRows = 52;                 // tensors and hyper-parameter sets per prologue launch: what 4 KB of kernel
+constexpr int kPrepRows = 104;                // tensors and hyper-parameter sets per prologue launch: what 4 KB of kernel
 constexpr int kPrepGroups = 8;                // arguments hold
 constexpr int kPrepThreads = 1024;
-constexpr int kNormThreads = 1024;
+constexpr long kNormChunk = 4096;             // the smallest number of elements a workgroup sums
 constexpr int kNormTable = 160;               // tensors per launch of the norm's first pass
 constexpr int kFinishWaves = 4;               // tensors per workgroup of the norm's second pass
-constexpr int kFirstTable = 1000;
+constexpr int kFirstTable = 1000;             // tensors per launch of that
 
 // what one tensor's update needs, computed once per step by the prologue
 struct OptCoef {
@@ -45,11 +45,12 @@ struct OptRow {
   long numel;
 };
 
+// A row on its way, in 32 bytes: addresses as differences from those of the launch's first row, parameters and gradients
+// in units of 2 bytes, the others of 4.  A tensor that is too far away starts another launch.
 struct PrepRow {
-  OptRow row;
-  float* step;
-  unsigned first;                             // first workgroup of the tensor within its launch
-  unsigned group;
+  int param, grad, m, v, scales, step;
+  unsigned numel;                             // lower 32 bits
+  unsigned first;                             // first workgroup of the tensor within its launch (24 bits), group (3), numel (5)
 };
 
 struct PrepGroup {
@@ -67,6 +68,8 @@ struct PrepTable {
   OptRow* rows;
   OptCoef* coef;
   unsigned* first;
+  OptRow base;
+  float* step_base;
   PrepGroup g[kPrepGroups];
   PrepRow row[kPrepRows];
 };
@@ -80,9 +83,15 @@ struct NormTable {
   unsigned first[kNormTable];
 };
 
-struct FirstTable { int n; unsigned v[kFirstTable]; };
+struct FinishTable {
+  int n, n_partial;
+  const double* partial;
+  float* total;                               // NULL: another launch writes it
+  float* each;
+  unsigned first[kFirstTable + 1];            // first partial sum of each tensor, and the end
+};
 
-static_assert(sizeof(PrepTable) <= 4096 && sizeof(NormTable) <= 4096 && sizeof(FirstTable) <= 4096, "kernel arguments");
+static_assert(sizeof(PrepTable) <= 4096 && sizeof(NormTable) <= 4096 && sizeof(FinishTable) <= 4096, "kernel arguments");
 
 template <typename T> __device__ inline float to_float(T x) { return (float)x; }
 template <typename T> __device__ inline T from_float(float x) { return (T)x; }   // round to nearest even
@@ -400,10 +409,10 @@ __device__ inline double wave_sum(double x) {
 }
 
 // 16 bytes a thread and load, four of them in flight
-template <bool kStream, typename T>
+template <int kThreads, bool kStream, typename T>
 __device__ inline double sum_squares(const T* __restrict__ g, long base, long end) {
   constexpr int N = 16 / sizeof(T);
-  constexpr long kRow = (long)N * kNormThreads;
+  constexpr long kRow = (long)N * kThreads;
   double s0 = 0.0, s1 = 0.0;
   long i = base + N * threadIdx.x;
   for (; i + 3 * kRow + N <= end; i += 4 * kRow) {
@@ -435,23 +444,23 @@ __device__ inline double sum_squares(const T* __restrict__ g, long base, long en
   return s0 + s1;
 }
 
-template <bool kStream>
-__global__ void __launch_bounds__(kNormThreads)
+template <int kThreads, bool kStream>
+__global__ void __launch_bounds__(kThreads)
 norm_partial_kernel(const NormTable tab) {
-  __shared__ double part[kNormThreads / 64];
+  __shared__ double part[kThreads / 64];
   const int k = find_tensor(tab.first, tab.n, blockIdx.x);
   const long base = (long)(blockIdx.x - tab.first[k]) * tab.chunk, numel = tab.numel[k] >> 2;
   const long end = base + tab.chunk < numel ? base + tab.chunk : numel;
   const int dtype = tab.numel[k] & 3;
   double s;
-  if (dtype == PIR_F32) s = sum_squares<kStream>((const float*)tab.grad[k], base, end);
-  else if (dtype == PIR_BF16) s = sum_squares<kStream>((const __bf16*)tab.grad[k], base, end);
-  else s = sum_squares<kStream>((const _Float16*)tab.grad[k], base, end);
+  if (dtype == PIR_F32) s = sum_squares<kThreads, kStream>((const float*)tab.grad[k], base, end);
+  else if (dtype == PIR_BF16) s = sum_squares<kThreads, kStream>((const __bf16*)tab.grad[k], base, end);
+  else s = sum_squares<kThreads, kStream>((const _Float16*)tab.grad[k], base, end);
   s = wave_sum(s);
   if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = s;
   __syncthreads();
   if (threadIdx.x != 0) return;
-  for (int w = 1; w < kNormThreads / 64; ++w) s += part[w];
+  for (int w = 1; w < kThreads / 64; ++w) s += part[w];
   tab.partial[blockIdx.x] = s;
 }
 
@@ -495,8 +504,9 @@ adamw_prologue_kernel(const PrepTable tab) {
   const int i = threadIdx.x;
   if (i >= tab.n) return;
   const PrepRow& r = tab.row[i];
-  const PrepGroup& g = tab.g[r.group];
-  const float t = *r.step + 1.0f;
+  const PrepGroup& g = tab.g[r.first >> 24 & 7];
+  float* step = tab.step_base + r.step;
+  const float t = *step + 1.0f;
   const double lr = g.lr_device ? (double)*g.lr_device : g.lr;
   OptCoef c;
   c.b1 = g.b1;
@@ -511,34 +521,38 @@ adamw_prologue_kernel(const PrepTable tab) {
   c.run = run ? 1.0f : 0.0f;
   c.pad0 = c.pad1 = 0.0f;
   tab.coef[tab.row0 + i] = c;
-  tab.rows[tab.row0 + i] = r.row;
-  tab.first[tab.row0 + i] = r.first;
-  if (run) *r.step = t;
+  OptRow row;
+  row.param = (short*)tab.base.param + r.param;
+  row.grad = (const short*)tab.base.grad + r.grad;
+  row.m = (int*)tab.base.m + r.m;
+  row.v = (int*)tab.base.v + r.v;
+  row.scales = tab.base.scales + r.scales;
+  row.numel = (long)(r.first >> 27) << 32 | r.numel;
+  tab.rows[tab.row0 + i] = row;
+  tab.first[tab.row0 + i] = r.first & 0xffffffu;
+  if (run) *step = t;
 }
 
-__global__ void write_first_kernel(const FirstTable tab, unsigned* out) {
-  for (int i = threadIdx.x; i < tab.n; i += kOptThreads) out[i] = tab.v[i];
-}
-
-// norms of all tensors together (workgroup 0) and of each (a wave each, in the others), from the partial sums
+// norms of all tensors together (workgroup 0 of the first launch) and of each (a wave each, in the others), from the
+// partial sums
 __global__ void __launch_bounds__(kPrepThreads)
-norm_finish_kernel(int n, const unsigned* __restrict__ first, int n_partial, const double* __restrict__ partial,
-                   float* __restrict__ total, float* __restrict__ each) {
+norm_finish_kernel(const FinishTable tab) {
   __shared__ double part[kPrepThreads / 64];
-  if (blockIdx.x == 0) {
-    const double all = sum_partials(partial, n_partial, part);
-    if (threadIdx.x == 0) *total = (float)sqrt(all);
-    return;
+  int group = blockIdx.x;
+  if (tab.total) {
+    if (group == 0) {
+      const double all = sum_partials(tab.partial, tab.n_partial, part);
+      if (threadIdx.x == 0) *tab.total = (float)sqrt(all);
+      return;
+    }
+    --group;
   }
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  if (wave >= kFinishWaves) return;
-  const int k = (blockIdx.x - 1) * kFinishWaves + wave;
-  if (k >= n) return;
-  const int end = k + 1 < n ? (int)first[k + 1] : n_partial;
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, k = group * kFinishWaves + wave;
+  if (wave >= kFinishWaves || k >= tab.n) return;
   double x = 0.0;
-  for (int i = first[k] + lane; i < end; i += 64) x += partial[i];
+  for (unsigned i = tab.first[k] + lane; i < tab.first[k + 1]; i += 64) x += tab.partial[i];
   x = wave_sum(x);
-  if (lane == 0) each[k] = (float)sqrt(x);
+  if (lane == 0) tab.each[k] = (float)sqrt(x);
 }
 
 static inline long ceil_div(long a, long b) { return (a + b - 1) / b; }
@@ -546,13 +560,15 @@ static inline long ceil_div(long a, long b) { return (a + b - 1) / b; }
 static const long kMaxGroups = (1L << 24) - 1;     // workgroups: a grid has fewer than 2^32 threads
 static const long kCacheBytes = 256L << 20;        // last-level cache
 
+static inline long element_bytes(int dtype) { return dtype == PIR_F32 ? 4 : 2; }
+
 // scales[i]: whether tensor i has 8-bit moments (scales NULL: none has)
 static int check_tensors(int n, const long* numels, const int* dtypes, const void* const* grads, float* const* scales) {
   if (n < 0 || (n > 0 && (!numels || !dtypes || !grads))) return PIR_ERR_ARG;
   long groups = 0;
   for (int i = 0; i < n; ++i) {
     if (numels[i] < 0 || dtypes[i] < PIR_F32 || dtypes[i] > PIR_F16) return PIR_ERR_ARG;
-    if (numels[i] > 0 && !grads[i]) return PIR_ERR_ARG;
+    if ((numels[i] > 0 && !grads[i]) || ((size_t)grads[i] & (element_bytes(dtypes[i]) - 1))) return PIR_ERR_ARG;
     if (numels[i] > kMaxGroups * kOptChunk8) return PIR_ERR_TOO_LARGE;
     groups += ceil_div(numels[i], scales && scales[i] ? kOptChunk8 : kOptChunk);
     if (groups > kMaxGroups) return PIR_ERR_TOO_LARGE;
@@ -560,14 +576,13 @@ static int check_tensors(int n, const long* numels, const int* dtypes, const voi
   return PIR_OK;
 }
 
-static inline long element_bytes(int dtype) { return dtype == PIR_F32 ? 4 : 2; }
-
-// Elements a workgroup takes: as few as fill the card when there is little to do, more of them when there is much, so
-// that the search for its tensor and the second pass over the partial sums stay small beside it.
+// Elements a workgroup takes: as few as fill the card when there is little to do (4096 for 256 threads: 4.5 us for 2.4 M
+// fp32 elements, 6.9 with 1024 threads), more of them when there is much, so that the search for its tensor and the second
+// pass over the partial sums stay small beside it (65536 for 1024 threads: 164 us for 284 M, 6.9 TB/s; with 256 threads 190).
 static unsigned norm_chunk(int n, const long* numels) {
   long total = 0;
   for (int i = 0; i < n; ++i) total += numels[i];
-  long chunk = 4096;
+  long chunk = kNormChunk;
   while (chunk < 65536 && total / chunk > 4096) chunk *= 2;
   return (unsigned)chunk;
 }
@@ -590,9 +605,10 @@ static int launch_partials(int n, const void* const* grads, const long* numels, 
   for (int i = 0; i <= n; ++i) {
     const long blocks = i < n ? ceil_div(numels[i], tab.chunk) : 0;
     if (tab.n > 0 && (i == n || tab.n == kNormTable)) {
-      const dim3 grid((unsigned)at), block(kNormThreads);
-      if (bytes > kCacheBytes) hipLaunchKernelGGL(norm_partial_kernel<true>, grid, block, 0, stream, tab);
-      else hipLaunchKernelGGL(norm_partial_kernel<false>, grid, block, 0, stream, tab);
+      const dim3 grid((unsigned)at);
+      if (bytes > kCacheBytes) hipLaunchKernelGGL((norm_partial_kernel<1024, true>), grid, dim3(1024), 0, stream, tab);
+      else if (tab.chunk > kNormChunk) hipLaunchKernelGGL((norm_partial_kernel<1024, false>), grid, dim3(1024), 0, stream, tab);
+      else hipLaunchKernelGGL((norm_partial_kernel<256, false>), grid, dim3(256), 0, stream, tab);
       tab.partial += at;
       tab.n = 0;
       at = 0;
@@ -618,6 +634,42 @@ static void launch_update(int kind, const UpdateArgs& args, long groups, hipStre
     case 3 + PIR_BF16: hipLaunchKernelGGL((adamw8_kernel<__bf16, kStream>), grid, block, 0, stream, args); break;
     default: hipLaunchKernelGGL((adamw8_kernel<_Float16, kStream>), grid, block, 0, stream, args);
   }
+}
+
+static PrepGroup prologue_group(const PirAdamwGroup& g) {
+  PrepGroup d;
+  d.lr = g.lr;
+  d.lr_device = g.lr_device;
+  d.log1 = std::log(g.beta1);
+  d.log2 = std::log(g.beta2);
+  d.wd = g.weight_decay;
+  d.b1 = (float)g.beta1;
+  d.c1 = (float)(1.0 - g.beta1);
+  d.b2 = (float)g.beta2;
+  d.c2 = (float)(1.0 - g.beta2);
+  d.eps = (float)g.eps;
+  d.pad = 0.0f;
+  return d;
+}
+
+// to - from in units of 1 << shift bytes; whether it fits
+static inline bool difference(const void* to, const void* from, int shift, int& d) {
+  const long x = ((long)to - (long)from) >> shift;
+  d = (int)x;
+  return x == d;
+}
+
+// the row's addresses as differences from the launch's; false: some do not fit.  An empty tensor has none that count, and
+// a launch whose first tensor is empty takes no others but such.
+static bool relative(const OptRow& row, const float* step, const PrepTable& tab, PrepRow& r) {
+  r.param = r.grad = r.m = r.v = r.scales = 0;
+  if (!difference(step, tab.step_base, 2, r.step)) return false;
+  if (row.numel == 0) return true;
+  if (tab.base.numel == 0) return false;
+  if (!difference(row.param, tab.base.param, 1, r.param) || !difference(row.grad, tab.base.grad, 1, r.grad) ||
+      !difference(row.m, tab.base.m, 2, r.m) || !difference(row.v, tab.base.v, 2, r.v))
+    return false;
+  return !row.scales || difference(row.scales, tab.base.scales, 2, r.scales);
 }
 
 static long align16(long x) { return (x + 15) & ~15L; }
@@ -661,6 +713,8 @@ int pir_adamw_step(int n, void* const* params, const void* const* grads, void* c
   for (int i = 0; i < n; ++i) {
     if (!steps[i] || groups[i] < 0 || groups[i] >= n_groups) return PIR_ERR_ARG;
     if (numels[i] > 0 && (!params[i] || !exp_avgs[i] || !exp_avg_sqs[i])) return PIR_ERR_ARG;
+    if (((size_t)params[i] & (element_bytes(dtypes[i]) - 1)) || (((size_t)exp_avgs[i] | (size_t)exp_avg_sqs[i] | (size_t)steps[i]) & 3))
+      return PIR_ERR_ARG;
     if (scales && scales[i] && ((((size_t)exp_avgs[i] | (size_t)exp_avg_sqs[i]) & 15) || ((size_t)scales[i] & 7)))
       return PIR_ERR_ARG;
   }
@@ -690,9 +744,10 @@ int pir_adamw_step(int n, void* const* params, const void* const* grads, void* c
   tab.rows = rows;
   tab.coef = coef;
   tab.first = first;
+  tab.base.scales = nullptr;
   int ids[kPrepGroups];
   auto prologue = [&]() {
-    hipLaunchKernelGGL(adamw_prologue_kernel, dim3(1), dim3(tab.norm && tab.finalize ? kPrepThreads : 64), 0, stream, tab);
+    hipLaunchKernelGGL(adamw_prologue_kernel, dim3(1), dim3(tab.norm && tab.finalize ? kPrepThreads : 128), 0, stream, tab);
     tab.row0 += tab.n;
     tab.n = tab.n_groups = tab.finalize = 0;
   };
@@ -703,38 +758,27 @@ int pir_adamw_step(int n, void* const* params, const void* const* grads, void* c
     kinds[kind].groups = 0;
     for (int i = 0; i < n; ++i) {
       if (dtypes[i] + (scales && scales[i] ? 3 : 0) != kind) continue;
+      const OptRow row = {params[i], grads[i], exp_avgs[i], exp_avg_sqs[i], kind >= 3 ? scales[i] : nullptr, numels[i]};
       int j = 0;
       while (j < tab.n_groups && ids[j] != groups[i]) ++j;
-      if (tab.n == kPrepRows || (j == tab.n_groups && j == kPrepGroups)) {
+      PrepRow r;
+      if (!tab.base.scales) tab.base.scales = row.scales;
+      if (tab.n == kPrepRows || j == kPrepGroups || (tab.n > 0 && !relative(row, steps[i], tab, r))) {
         prologue();
         j = 0;
       }
-      if (j == tab.n_groups) {
-        const PirAdamwGroup& g = group[groups[i]];
-        PrepGroup& d = tab.g[j];
-        ids[tab.n_groups++] = groups[i];
-        d.lr = g.lr;
-        d.lr_device = g.lr_device;
-        d.log1 = std::log(g.beta1);
-        d.log2 = std::log(g.beta2);
-        d.wd = g.weight_decay;
-        d.b1 = (float)g.beta1;
-        d.c1 = (float)(1.0 - g.beta1);
-        d.b2 = (float)g.beta2;
-        d.c2 = (float)(1.0 - g.beta2);
-        d.eps = (float)g.eps;
-        d.pad = 0.0f;
+      if (tab.n == 0) {
+        tab.base = row;
+        tab.step_base = steps[i];
+        relative(row, steps[i], tab, r);
       }
-      PrepRow& r = tab.row[tab.n++];
-      r.row.param = params[i];
-      r.row.grad = grads[i];
-      r.row.m = exp_avgs[i];
-      r.row.v = exp_avg_sqs[i];
-      r.row.scales = kind >= 3 ? scales[i] : nullptr;
-      r.row.numel = numels[i];
-      r.step = steps[i];
-      r.first = (unsigned)kinds[kind].groups;
-      r.group = (unsigned)j;
+      if (j == tab.n_groups) {
+        ids[tab.n_groups++] = groups[i];
+        tab.g[j] = prologue_group(group[groups[i]]);
+      }
+      r.numel = (unsigned)numels[i];
+      r.first = (unsigned)kinds[kind].groups | (unsigned)j << 24 | (unsigned)(numels[i] >> 32) << 27;
+      tab.row[tab.n++] = r;
       kinds[kind].groups += ceil_div(numels[i], kind >= 3 ? kOptChunk8 : kOptChunk);
       ++kinds[kind].n;
     }
@@ -752,7 +796,7 @@ int pir_adamw_step(int n, void* const* params, const void* const* grads, void* c
 
 size_t pir_grad_norm_workspace_bytes(int n, const long* numels) {
   if (n < 0 || (n > 0 && !numels)) return 0;
-  return 8 * (size_t)norm_partials(n, numels) + 4 * ((size_t)n + 1);
+  return 8 * (size_t)norm_partials(n, numels) + 8;
 }
 
 int pir_grad_norm(int n, const void* const* grads, const long* numels, const int* dtypes, float* total, float* each,
@@ -764,25 +808,26 @@ int pir_grad_norm(int n, const void* const* grads, const long* numels, const int
   if (!workspace || workspace_bytes < pir_grad_norm_workspace_bytes(n, numels)) return PIR_ERR_SCRATCH;
   const long n_partial = norm_partials(n, numels);
   double* partial = (double*)workspace;
-  unsigned* first = (unsigned*)(partial + n_partial);
   if (launch_partials(n, grads, numels, dtypes, partial, stream) != PIR_OK) return PIR_ERR_LAUNCH;
-  if (each) {
-    const unsigned chunk = norm_chunk(n, numels);
-    FirstTable tab;
-    long at = 0;
+  const unsigned chunk = norm_chunk(n, numels);
+  FinishTable tab;
+  tab.n_partial = (int)n_partial;
+  tab.partial = partial;
+  tab.total = total;
+  long at = 0;
+  int i = 0;
+  do {
     tab.n = 0;
-    for (int i = 0; i < n; ++i) {
-      tab.v[tab.n++] = (unsigned)at;
+    tab.each = each ? each + i : nullptr;
+    tab.first[0] = (unsigned)at;
+    for (; each && i < n && tab.n < kFirstTable; ++i) {
       at += ceil_div(numels[i], chunk);
-      if (tab.n == kFirstTable || i == n - 1) {
-        hipLaunchKernelGGL(write_first_kernel, dim3(1), dim3(kOptThreads), 0, stream, tab, first + (i + 1 - tab.n));
-        tab.n = 0;
-      }
+      tab.first[++tab.n] = (unsigned)at;
     }
-  }
-  const unsigned waves = each ? (unsigned)ceil_div(n, kFinishWaves) : 0;
-  hipLaunchKernelGGL(norm_finish_kernel, dim3(1 + waves), dim3(kPrepThreads), 0, stream, n, (const unsigned*)first,
-                     (int)n_partial, (const double*)partial, total, each);
+    const unsigned waves = (unsigned)ceil_div(tab.n, kFinishWaves);
+    hipLaunchKernelGGL(norm_finish_kernel, dim3((tab.total ? 1 : 0) + waves), dim3(kPrepThreads), 0, stream, tab);
+    tab.total = nullptr;
+  } while (each && i < n);
   return pir_check_launch();
 }
 

@@ -123,6 +123,7 @@ PyObject* step(PyObject*, PyObject* args) {
       const long numel = p->numel();
       const int type = dtype_of(*p);
       if (type < 0 || g->scalar_type() != p->scalar_type() || !dense(*p) || !same_layout(*p, *g)) Py_RETURN_NOTIMPLEMENTED;
+      if (((size_t)address(*p) | (size_t)address(*g)) & (p->element_size() - 1)) Py_RETURN_NOTIMPLEMENTED;
       char *am = address(*m), *av = address(*v), *as = nullptr;
       PyObject* so = ss == Py_None ? Py_None : S.at[i];
       if (so == Py_None) {
@@ -210,7 +211,8 @@ PyObject* norm(PyObject*, PyObject* args) {
     std::vector<int> dtypes(G.n);
     for (Py_ssize_t i = 0; i < G.n; ++i) {
       const at::Tensor* t = tensor_of(G.at[i], dev);
-      if (!t || (dtypes[i] = dtype_of(*t)) < 0 || !dense(*t)) Py_RETURN_NOTIMPLEMENTED;
+      if (!t || (dtypes[i] = dtype_of(*t)) < 0 || !dense(*t) || ((size_t)address(*t) & (t->element_size() - 1)))
+        Py_RETURN_NOTIMPLEMENTED;
       g[i] = address(*t);
       numels[i] = t->numel();
     }

@@ -118,6 +118,8 @@ def _check(params, grads, exp_avgs, exp_avg_sqs, scales):
             raise ValueError(f"gradient {i}: a dense tensor of its parameter's shape and type is wanted")
         if not (p.device == dev and g.device == dev and m.device == dev and v.device == dev):
             raise ValueError(f"tensors {i}: on another device than parameter 0")
+        if p.data_ptr() % p.element_size() or (g.data_ptr() % g.element_size() and _same_layout(p, g)):
+            raise ValueError(f"tensors {i}: their addresses are not multiples of their type's size")
         if not p.is_contiguous() and not _dense(p):
             raise ValueError(f"parameter {i}: its elements do not fill one stretch of memory (strides {p.stride()})")
         s = scales[i] if scales is not None else None
