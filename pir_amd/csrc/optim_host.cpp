@@ -125,6 +125,7 @@ PyObject* step(PyObject*, PyObject* args) {
       if (type < 0 || g->scalar_type() != p->scalar_type() || !dense(*p) || !same_layout(*p, *g)) Py_RETURN_NOTIMPLEMENTED;
       if (((size_t)address(*p) | (size_t)address(*g)) & (p->element_size() - 1)) Py_RETURN_NOTIMPLEMENTED;
       char *am = address(*m), *av = address(*v), *as = nullptr;
+      if (numel && (am == av || am == address(*p) || av == address(*p))) Py_RETURN_NOTIMPLEMENTED;
       PyObject* so = ss == Py_None ? Py_None : S.at[i];
       if (so == Py_None) {
         if (m->scalar_type() != at::kFloat || v->scalar_type() != at::kFloat || !same_layout(*p, *m) || !same_layout(*p, *v))

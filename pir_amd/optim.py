@@ -122,6 +122,8 @@ def _check(params, grads, exp_avgs, exp_avg_sqs, scales):
             raise ValueError(f"tensors {i}: their addresses are not multiples of their type's size")
         if not p.is_contiguous() and not _dense(p):
             raise ValueError(f"parameter {i}: its elements do not fill one stretch of memory (strides {p.stride()})")
+        if p.numel() and len({p.data_ptr(), m.data_ptr(), v.data_ptr()}) < 3:
+            raise ValueError(f"tensors {i}: one of them is given twice")
         s = scales[i] if scales is not None else None
         if s is None:
             if m.dtype != torch.float32 or v.dtype != torch.float32 or not (_same_layout(p, m) and _same_layout(p, v)):
@@ -371,6 +373,9 @@ class AdamW(torch.optim.Optimizer):
             self.param_groups.pop()
             raise
 
+    def __getstate__(self):
+        return {**super().__getstate__(), "max_norm": self.max_norm, "skip_nonfinite": self.skip_nonfinite, "total_norm": None}
+
     def __setstate__(self, state):
         super().__setstate__(state)
         for g in self.param_groups:
@@ -441,32 +446,47 @@ def step_together(optimizers, max_norm=None, skip_nonfinite=False):
     """One step of several AdamW optimizers in one call, their gradients clipped to one joint norm.  (The optimizers' own
     max_norm and skip_nonfinite are for their own step().)  Returns the joint norm with max_norm or skip_nonfinite."""
     bound = _max_norm(max_norm)
-    by_device = {}
+    jobs = {}                    # device -> its tensors, of all optimizers
     for opt in optimizers:
         if not isinstance(opt, AdamW):
             raise TypeError(f"step_together takes pir_amd.optim.AdamW optimizers, not {type(opt).__name__}")
         for group in opt.param_groups:
             live = [p for p in group["params"] if p.grad is not None]
-            for dev in {p.device for p in live}:
-                job = by_device.setdefault(dev, ([], [], []))
-                mine = [p for p in live if p.device == dev]
-                job[0].extend(mine)
-                job[1].extend([len(job[2])] * len(mine))
-                job[2].append((opt, group))
-    if len(by_device) > 1 and (bound or skip_nonfinite):
+            places = {p.get_device() for p in live}
+            for place in places:
+                mine = live if len(places) == 1 else [p for p in live if p.get_device() == place]
+                states = [opt.state[p] for p in mine]
+                if not all(states):
+                    states = [opt._state_of(p, group) for p in mine]
+                job = jobs.setdefault(place, _Job(mine[0].device))
+                job.add(mine, states, _hyper(group["lr"], group["betas"], group["eps"], group["weight_decay"], job.device))
+    if len(jobs) > 1 and (bound or skip_nonfinite):
         raise ValueError("a joint norm of parameters on several devices is not supported")
     norm = torch.zeros(()) if max_norm is not None or skip_nonfinite else None      # what no gradients have
-    for dev, (params, index, owners) in by_device.items():
-        hypers = [_hyper(g["lr"], g["betas"], g["eps"], g["weight_decay"], dev) for _, g in owners]
-        if dev.type != "cuda" and any(h[5] for h in hypers):
-            raise ValueError("lr: on another device than the parameters")
-        states = [owners[k][0]._state_of(p, owners[k][1]) for p, k in zip(params, index)]
-        m, v, t = ([s[k] for s in states] for k in ("exp_avg", "exp_avg_sq", "step"))
-        scales = [s.get("scales") for s in states]
-        grads = [p.grad for p in params]
-        if dev.type == "cuda":
-            norm = _run(params, grads, m, v, scales, t, array("i", index), hypers, bound, skip_nonfinite, max_norm is not None)
-        else:
-            grads = _check(params, grads, m, v, scales)
-            norm = _run_torch(params, grads, m, v, scales, t, index, hypers, bound, skip_nonfinite, max_norm is not None)
+    for job in jobs.values():
+        norm = job.run(bound, skip_nonfinite, max_norm is not None)
     return norm
+
+
+class _Job:
+    """The tensors of one device in a step of one or more optimizers."""
+
+    def __init__(self, device):
+        self.device, self.params, self.states, self.groups, self.hypers = device, [], [], array("i"), []
+
+    def add(self, params, states, hyper):
+        if hyper[5] and self.device.type != "cuda":
+            raise ValueError("lr: on another device than the parameters")
+        self.params += params
+        self.states += states
+        self.groups.extend([len(self.hypers)] * len(params))
+        self.hypers.append(hyper)
+
+    def run(self, bound, skip_nonfinite, want_norm):
+        grads = [p.grad for p in self.params]
+        m, v, t = ([s[k] for s in self.states] for k in ("exp_avg", "exp_avg_sq", "step"))
+        scales = [s.get("scales") for s in self.states]
+        rest = (t, self.groups, self.hypers, bound, skip_nonfinite, want_norm)
+        if self.device.type == "cuda":
+            return _run(self.params, grads, m, v, scales, *rest)
+        return _run_torch(self.params, _check(self.params, grads, m, v, scales), m, v, scales, *rest)

@@ -47,6 +47,8 @@ def lists(n=300, bits=32, count=2):
     ("a parameter that is one element, expanded", dict(params=lambda x: [x[0], torch.zeros(1).expand(300)])),
     ("a parameter twice", dict(params=lambda x: [x[0], x[0]])),
     ("parameters that overlap", dict(params=lambda x: (lambda b: [b[:300], b[299:599]])(torch.zeros(599)))),
+    ("one list for both moments", dict(exp_avg_sqs=lambda x: "exp_avgs")),
+    ("the parameters for a moment", dict(exp_avgs=lambda x: "params")),
     ("a moment twice", dict(exp_avgs=lambda x: [x[1], x[1]])),
     ("a moment of another type", dict(exp_avg_sqs=lambda x: [x[0], x[1].bfloat16()])),
     ("a moment of another shape", dict(exp_avgs=lambda x: [x[0], x[1].view(30, 10)])),
@@ -63,6 +65,7 @@ def test_step_refuses(what, change):
     before = {k: [t.clone() for t in args[k]] for k in ("params", "exp_avgs", "exp_avg_sqs")}
     for k, f in change.items():
         args[k] = f(args[k]) if callable(f) and k not in ("lr",) else f
+        args[k] = args[args[k]] if isinstance(args[k], str) else args[k]
     lists_only = {k: args.pop(k) for k in ("params", "grads", "exp_avgs", "exp_avg_sqs", "steps")}
     kept = lists(), before
     with pytest.raises(ValueError):
@@ -250,6 +253,17 @@ def test_load_state_dict(source, bits):
     if bits == 32:
         back.load_state_dict(second.state_dict())        # and torch takes it back
         assert float(list(back.state.values())[0]["step"]) == 5
+
+
+def test_copies_of_the_optimizer_keep_its_settings():
+    import copy
+    net = networks()
+    opt = copy.deepcopy(optim.AdamW(net.parameters(), max_norm=0.5, skip_nonfinite=True, state_bits=8))
+    for g in opt.param_groups:
+        for p in g["params"]:
+            p.grad = torch.ones_like(p)
+    opt.step()
+    assert opt.max_norm == 0.5 and opt.skip_nonfinite and float(opt.total_norm) > 1 and opt.param_groups[0]["state_bits"] == 8
 
 
 def test_load_state_dict_refuses():

@@ -29,7 +29,8 @@ ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 sys.path.insert(0, ROOT)
 
 
-def build_state(device, patch, stage, n_views=8, res=800, bumpy=True, handle_edges=True, smoothness=1e-4):
+def build_state(device, patch, stage, n_views=8, res=800, bumpy=True, handle_edges=True, smoothness=1e-4,
+                optimizer="adam"):
     from pir_amd import scene, train
     from pir_amd.render_fn import make_render_fn
     from pir_amd.renderer.raytracer import RayTracer
@@ -47,7 +48,8 @@ def build_state(device, patch, stage, n_views=8, res=800, bumpy=True, handle_edg
     cfg = train.TrainConfig(num_iters=50001, patch_size=patch, render_visibility=(stage == 2),
                             render_brdf=(stage == 3), smoothness_weight=smoothness, handle_edges=handle_edges)
     lr = dict(scene.MODEL_CONFIG["lr"], dino_network=1e-3)
-    sdf_opt, color_opts, dino_opt = train.make_optimizers(sdf, nets, dino, lr, render_visibility=(stage == 2))
+    sdf_opt, color_opts, dino_opt = train.make_optimizers(sdf, nets, dino, lr, render_visibility=(stage == 2),
+                                                             optimizer=optimizer)
     cams = [scene.make_camera(res, res, view=v, n_views=n_views, device=dev) for v in range(n_views)]
     g = torch.Generator().manual_seed(2)
     gt = torch.rand(n_views, res, res, 3, generator=g).to(dev)
@@ -83,11 +85,12 @@ def main():
     ap.add_argument("--global-step", type=int, default=12000)
     ap.add_argument("--no-edges", action="store_true")
     ap.add_argument("--threads", type=int, default=0)
+    ap.add_argument("--optimizer", default="adam", choices=["adam", "adamw", "adamw8"])
     args = ap.parse_args()
     if args.threads:
         torch.set_num_threads(args.threads)
     dev = torch.device(args.device)
-    state = build_state(dev, args.patch, args.stage, handle_edges=not args.no_edges)
+    state = build_state(dev, args.patch, args.stage, handle_edges=not args.no_edges, optimizer=args.optimizer)
     from pir_amd import train
     from pir_amd.renderer.raytracer import Camera
     # the timed steps always see the same crops and views, whatever the warm-up length (warm-up cycles through them too)
@@ -129,7 +132,7 @@ def main():
         sync()
     hits, edges = int(hits), int(edges)
     rays = args.patch * args.patch * args.steps
-    print(json.dumps({"tool": "bench_train_patch", "device": str(dev), "stage": args.stage, "patch": args.patch,
+    print(json.dumps({"tool": "bench_train_patch", "device": str(dev), "stage": args.stage, "patch": args.patch, "optimizer": args.optimizer,
                       "steps": args.steps, "warmup": args.warmup, "global_step": args.global_step,
                       "handle_edges": not args.no_edges, "indirect": args.global_step >= 10000,
                       "it_per_s": round(args.steps / dt, 3), "rays_per_s": round(rays / dt, 1),
