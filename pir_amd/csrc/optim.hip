@@ -99,7 +99,9 @@ template <typename T> __device__ inline T from_float(float x) { return (T)x; }  
 // N values of type T at any address that is a multiple of sizeof(T): one wide access all the same
 template <typename T, int N> struct Vec { typedef T type __attribute__((ext_vector_type(N), aligned(sizeof(T)))); };
 
-// kStream: data that is too much for the last-level cache passes it by
+// kStream: accesses that leave the caches to others, where the call's data exceeds the last-level one.  284 M fp32 elements
+// take 1.41 ms with them, 1.51 without; 7.3 M with 8-bit moments (117 MB, which the next call finds in the cache) 55.5 us
+// with them, 51.5 without.
 template <bool kStream, typename T, int N>
 __device__ inline void load(float (&x)[N], const T* __restrict__ p) {
   const typename Vec<T, N>::type* q = (const typename Vec<T, N>::type*)p;
@@ -132,18 +134,6 @@ __device__ inline int find_tensor(const unsigned* first, int n, unsigned block) 
   return __builtin_amdgcn_readfirstlane(lo);
 }
 
-struct Updated { float p, m, v; };
-
-__device__ inline Updated adamw_element(const OptCoef& c, float p, float g, float m, float v) {
-  g *= c.gscale;
-  Updated r;
-  r.m = fmaf(c.b1, m, c.c1 * g);
-  r.v = fmaf(c.b2, v, c.c2 * g * g);
-  const float u = r.m / fmaf(sqrtf(r.v), c.root, c.eps);
-  r.p = p - fmaf(c.decay, p, c.size * u);
-  return r;
-}
-
 struct UpdateArgs {
   const OptRow* rows;
   const OptCoef* coef;
@@ -151,64 +141,60 @@ struct UpdateArgs {
   int n;
 };
 
-// 32-bit moments: 28 bytes an element in fp32, 22 in 16 bits, bound by memory.  A workgroup has two groups of 4
-// consecutive elements a thread, all of whose loads are in flight before the first is used.
+// 32-bit moments, 4 consecutive elements a thread and no loop: 28 bytes an element in fp32, 22 in 16 bits, bound by memory.
+// 284 M fp32 elements: 1.31 ms, 6.1 TB/s; 88 M bf16: 0.29 ms, 6.6 TB/s.  What a workgroup covers decides how near to each
+// other the card's accesses lie: with 32768, 8192 and 2048 elements a workgroup the fp32 step took 1.60, 1.54 and 1.51 ms,
+// with streaming accesses 1.47 (8192), 1.41 (2048) and 1.34 (1024, as here; 512: 1.35).
 template <typename T, bool kStream>
 __global__ void __launch_bounds__(kOptThreads)
 adamw32_kernel(const UpdateArgs args) {
+  static_assert(kOptChunk == 4 * kOptThreads, "4 elements a thread");
   const int k = find_tensor(args.first, args.n, blockIdx.x);
   const OptCoef c = args.coef[k];
   if (c.run == 0.0f) return;
   const OptRow t = args.rows[k];
-  const long base = (long)(blockIdx.x - args.first[k]) * kOptChunk, end = t.numel;
+  const long end = t.numel, i = (long)(blockIdx.x - args.first[k]) * kOptChunk + 4 * threadIdx.x;
   T* __restrict__ P = (T*)t.param;
   const T* __restrict__ G = (const T*)t.grad;
   float* __restrict__ M = (float*)t.m;
   float* __restrict__ V = (float*)t.v;
-  constexpr int kQuads = kOptChunk / (4 * kOptThreads);
-  float p[kQuads][4], g[kQuads][4], m[kQuads][4], v[kQuads][4];
+  const bool whole = i + 4 <= end;
+  float p[4], g[4], m[4], v[4];
+  if (whole) {
+    load<kStream>(p, P + i);
+    load<kStream>(g, G + i);
+    load<kStream>(m, M + i);
+    load<kStream>(v, V + i);
+  } else {
 #pragma unroll
-  for (int h = 0; h < kQuads; ++h) {
-    const long i = base + 4 * (h * kOptThreads + threadIdx.x);
-    if (i + 4 <= end) {
-      load<kStream>(p[h], P + i);
-      load<kStream>(g[h], G + i);
-      load<kStream>(m[h], M + i);
-      load<kStream>(v[h], V + i);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const bool in = i + j < end;
-        p[h][j] = in ? to_float(P[i + j]) : 0.0f;
-        g[h][j] = in ? to_float(G[i + j]) : 0.0f;
-        m[h][j] = in ? M[i + j] : 0.0f;
-        v[h][j] = in ? V[i + j] : 0.0f;
-      }
+    for (int j = 0; j < 4; ++j) {
+      const bool in = i + j < end;
+      p[j] = in ? to_float(P[i + j]) : 0.0f;
+      g[j] = in ? to_float(G[i + j]) : 0.0f;
+      m[j] = in ? M[i + j] : 0.0f;
+      v[j] = in ? V[i + j] : 0.0f;
     }
   }
 #pragma unroll
-  for (int h = 0; h < kQuads; ++h) {
-    const long i = base + 4 * (h * kOptThreads + threadIdx.x);
+  for (int j = 0; j < 4; ++j) {
+    const float gj = g[j] * c.gscale;
+    m[j] = fmaf(c.b1, m[j], c.c1 * gj);
+    v[j] = fmaf(c.b2, v[j], c.c2 * gj * gj);
+    const float u = m[j] / fmaf(sqrtf(v[j]), c.root, c.eps);
+    p[j] -= fmaf(c.decay, p[j], c.size * u);  // the decay is added to the step: 1 - lr wd in fp32 would lose a small one
+  }
+  if (whole) {
+    store<kStream>(P + i, p);
+    store<kStream>(M + i, m);
+    store<kStream>(V + i, v);
+  } else {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const Updated r = adamw_element(c, p[h][j], g[h][j], m[h][j], v[h][j]);
-      p[h][j] = r.p;
-      m[h][j] = r.m;
-      v[h][j] = r.v;
-    }
-    if (i + 4 <= end) {
-      store<kStream>(P + i, p[h]);
-      store<kStream>(M + i, m[h]);
-      store<kStream>(V + i, v[h]);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (i + j < end) {
-          P[i + j] = from_float<T>(p[h][j]);
-          M[i + j] = m[h][j];
-          V[i + j] = v[h][j];
-        }
-    }
+    for (int j = 0; j < 4; ++j)
+      if (i + j < end) {
+        P[i + j] = from_float<T>(p[j]);
+        M[i + j] = m[j];
+        V[i + j] = v[j];
+      }
   }
 }
 
@@ -269,7 +255,9 @@ __device__ inline unsigned pack_low_bytes(float a, float b, float c, float d) {
 
 // 8-bit moments: half a wave per block of 256 elements, 8 consecutive ones per lane.  10 bytes an element (16-bit
 // parameters) leave the vector unit about 60 operations each, so the arithmetic is counted: square roots and reciprocals
-// are the hardware's (one ulp), the root of v serves the step and the new code, and codes are rounded and packed as bits.
+// are the hardware's (one ulp), the root of v serves the step and the new code, codes are rounded and packed as bits, and
+// maxima cross lanes without shared memory.  435 M bf16 elements: 0.68 ms, 6.5 TB/s, bound by memory; with IEEE roots and
+// divisions and shuffles through shared memory 1.51 ms.
 template <typename T, bool kStream>
 __global__ void __launch_bounds__(kOptThreads)
 adamw8_kernel(const UpdateArgs args) {
@@ -353,6 +341,7 @@ adamw8_kernel(const UpdateArgs args) {
   if ((threadIdx.x & 31) == 0) *sc = make_float2(na, nb);
 }
 
+// 435 M elements to bf16 (2.6 GB): 0.41 ms, 6.4 TB/s
 template <typename T>
 __global__ void __launch_bounds__(kOptThreads)
 moments8_decode_kernel(long n_blocks, const signed char* __restrict__ mq, const unsigned char* __restrict__ vq,
@@ -401,7 +390,8 @@ moments8_encode_kernel(long numel, const T* __restrict__ m, const T* __restrict_
 }
 
 // ---- norms: squares and sums in 64 bits (no overflow for any fp32 gradient), one partial sum per workgroup, added up
-// in a fixed order: the same bits on every run
+// in a fixed order: the same bits on every run.  Bound by memory (6.9 TB/s at 284 M fp32 elements).  Gradients that fit the
+// last-level cache are left there: the step reads them again (88 M bf16, clipped: 330 us, 352 with streaming reads).
 
 __device__ inline double wave_sum(double x) {
   for (int d = 32; d >= 1; d >>= 1) x += __shfl_xor(x, d);
@@ -477,7 +467,9 @@ __device__ inline double sum_partials(const double* __restrict__ partial, int n,
 }
 
 // One workgroup: the joint norm and clip factor from the partial sums, then the step counts and coefficients of its
-// tensors, and their descriptors for the update kernels.
+// tensors (in 64 bits: 1 - beta2^t at t = 1 loses three digits in 32), and their descriptors for the update kernels.  2.4 to
+// 4 us, nearly all of it the launch and one chain of dependent reads; it spares every workgroup of the update the 64-bit
+// exponentials, and a step of many tensors all but one update launch (301 tensors: 155 us with 64 tensors a launch, 49 so).
 __global__ void __launch_bounds__(kPrepThreads)
 adamw_prologue_kernel(const PrepTable tab) {
   __shared__ double part[kPrepThreads / 64];
@@ -715,7 +707,8 @@ int pir_adamw_step(int n, void* const* params, const void* const* grads, void* c
     if (numels[i] > 0 && (!params[i] || !exp_avgs[i] || !exp_avg_sqs[i])) return PIR_ERR_ARG;
     if (((size_t)params[i] & (element_bytes(dtypes[i]) - 1)) || (((size_t)exp_avgs[i] | (size_t)exp_avg_sqs[i] | (size_t)steps[i]) & 3))
       return PIR_ERR_ARG;
-    if (scales && scales[i] && ((((size_t)exp_avgs[i] | (size_t)exp_avg_sqs[i]) & 15) || ((size_t)scales[i] & 7)))
+    if (scales && scales[i] && ((((size_t)exp_avgs[i] | (size_t)exp_avg_sqs[i]) & 15) || ((size_t)scales[i] & 7) ||
+                                group[groups[i]].eps < 1e-30))
       return PIR_ERR_ARG;
   }
   const bool clip = max_norm > 0.0, with_norm = clip || skip_nonfinite || total_norm;

@@ -16,8 +16,8 @@ With t the step count of a tensor and g its gradient, times min(1, max_norm / (|
 
 computed in fp32 and rounded once to p's type (fp32, bf16 or fp16; gradients have the type of their parameter).  The 8-bit
 moments of 256 consecutive elements are m = a (q / 127) |q / 127| (int8 q) and v = b (c / 255)^4 (uint8 c) with a, b the
-block's largest |m| and v in fp32, rounded to the nearest code, except that a v above zero keeps c >= 1.  A block whose
-largest is below 2^-126 is zero; one that holds an infinity or a NaN has a scale of NaN, as that element would have
+block's largest |m| and v in fp32, rounded to the nearest code, except that a v above zero keeps c >= 1 (in a step: a v of
+2^-126 or more).  A block whose largest is below 2^-126 is zero; one that holds an infinity or a NaN has a scale of NaN, as that element would have
 moments of NaN in 32 bits: skip_nonfinite leaves everything as it is in such a step.
 
 Step counts live on the device (fp32, one per tensor), so that a step can be captured into a HIP graph and replayed; a
@@ -34,6 +34,7 @@ from . import _lib
 
 BLOCK = 256                      # elements that share a scale
 _TINY = 2.0 ** -126              # blocks whose largest is below this are zero
+_LEAST_EPS = 1e-30               # with 8-bit moments: their roots take what is below 2^-126 for zero
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
@@ -102,6 +103,11 @@ def _check_disjoint(what, tensors):
 
 def _same_layout(p, t):
     return t.shape == p.shape and (t.stride() == p.stride() or (t.is_contiguous() and p.is_contiguous()))
+
+
+def _check_eps(eps, coded):
+    if coded and eps < _LEAST_EPS:
+        raise ValueError(f"eps: at least {_LEAST_EPS} with 8-bit moments, not {eps}")
 
 
 def _check(params, grads, exp_avgs, exp_avg_sqs, scales):
@@ -224,6 +230,7 @@ def _step(params, grads, exp_avgs, exp_avg_sqs, scales, steps, lr, betas, eps, w
     want = max_norm is not None
     dev = steps.device
     hyper = _hyper(lr, betas, eps, weight_decay, dev)
+    _check_eps(hyper[3], scales is not None)
     if steps.dtype != torch.float32 or not steps.is_contiguous() or steps.numel() != len(params):
         raise ValueError("steps: a contiguous float32 tensor with one count per parameter")
     if not params:
@@ -389,6 +396,9 @@ class AdamW(torch.optim.Optimizer):
     def _state_of(self, p, group):
         s = self.state[p]
         if not s:
+            if p.is_cuda and torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("a parameter's first step cannot be captured: every replay would clear its moments; take "
+                                   "one step before the capture")
             s["step"] = torch.zeros((), dtype=torch.float32, device=p.device)
             if self._in_8_bits(p, group):
                 nb = _blocks(p.numel())
@@ -428,6 +438,12 @@ class AdamW(torch.optim.Optimizer):
         s = self._state_of(p, group)
         s["step"].fill_(step)
         put = {k: saved[k].detach().to(p.device) for k in ("exp_avg", "exp_avg_sq", "scales") if k in saved}
+        nb = _blocks(p.numel())
+        coded = {"exp_avg": (nb, BLOCK), "exp_avg_sq": (nb, BLOCK), "scales": (nb, 2)}
+        for k, x in put.items():
+            want = coded[k] if "scales" in put else tuple(p.shape)
+            if tuple(x.shape) != want:
+                raise ValueError(f"state {k}: {tuple(x.shape)} for a parameter of {tuple(p.shape)}")
         if "scales" in s and "scales" not in put:
             like = torch.empty_like(p, dtype=torch.float32, requires_grad=False)
             m, v = (like.clone().copy_(put[k]) for k in ("exp_avg", "exp_avg_sq"))
@@ -436,8 +452,6 @@ class AdamW(torch.optim.Optimizer):
             m, v = moments8_decode(*(put[k].contiguous() for k in ("exp_avg", "exp_avg_sq", "scales")))
             put = {k: x.reshape(-1)[:p.numel()].as_strided(p.shape, p.stride()) for k, x in (("exp_avg", m), ("exp_avg_sq", v))}
         for k, x in put.items():
-            if s[k].shape != x.shape:
-                raise ValueError(f"state {k}: {tuple(x.shape)} does not fit {tuple(s[k].shape)}")
             s[k].copy_(x)
 
 
@@ -477,6 +491,7 @@ class _Job:
     def add(self, params, states, hyper):
         if hyper[5] and self.device.type != "cuda":
             raise ValueError("lr: on another device than the parameters")
+        _check_eps(hyper[3], any("scales" in s for s in states))
         self.params += params
         self.states += states
         self.groups.extend([len(self.hypers)] * len(params))

@@ -237,15 +237,73 @@ def test_mixed_types_and_moments_in_one_call():
         assert ("scales" in opt.state[p]) == (i in (0, 1, 5))
 
 
-def test_more_groups_than_one_prologue_holds():
+@pytest.mark.parametrize("max_norm", [None, 1e3])
+def test_more_groups_than_one_prologue_holds(max_norm):
     ps = [torch.nn.Parameter(torch.ones(5, device=DEV)) for _ in range(40)]
-    opt = optim.AdamW([{"params": [p], "lr": 1e-3 * (i + 1)} for i, p in enumerate(ps)], weight_decay=0.0)
+    opt = optim.AdamW([{"params": [p], "lr": 1e-3 * (i + 1)} for i, p in enumerate(ps)], weight_decay=0.0, max_norm=max_norm)
     for p in ps:
         p.grad = torch.ones_like(p)
     opt.step()
     for i, p in enumerate(ps):                           # first step: lr times the sign of the gradient
-        assert float((1 - p - 1e-3 * (i + 1)).abs().max()) < 2e-7
+        assert float((1 - p.detach() - 1e-3 * (i + 1)).abs().max()) < 2e-7
     assert all(float(opt.state[p]["step"]) == 1 for p in ps)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_tensors_far_apart(bits):
+    """More than 8 GB between two tensors of a call, in either order: descriptors are differences of 32 bits."""
+    room = torch.empty(20 * 2 ** 30, dtype=torch.uint8, device=DEV).view(torch.float32)
+    hyper = dict(lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.1)
+    p, g, m, v, s, steps = U.make([5000] * 4, torch.float32, bits, DEV)
+    near = [t.clone() for t in p], g, [t.clone() for t in m], [t.clone() for t in v], None if s is None else [t.clone() for t in s], steps.clone()
+    at = [room.numel() - 5000, 0, room.numel() // 2, 5000]
+    far = [room[i:i + 5000].copy_(t) for i, t in zip(at, p)]
+    run(far, g, m, v, s, steps, 0.1, **hyper)
+    run(*near, 0.1, **hyper)
+    assert all(torch.equal(a, b) for a, b in zip(far, near[0])) and torch.equal(steps, near[5])
+    assert all(torch.equal(a, b) for a, b in zip(m, near[2])) and all(torch.equal(a, b) for a, b in zip(v, near[3]))
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_skipped_step_of_many_tensors(bits):
+    p, g, m, v, s, steps = U.make([40] * 300, torch.float32, bits, DEV)
+    before = [x.clone() for y in (p, m, v, s or []) for x in y] + [steps.clone()]
+    g[299][39] = -math.inf
+    norm = optim._step(p, g, m, v, s, steps, 1e-3, (0.9, 0.999), 1e-8, 0.0, None, True)
+    assert float(norm) == math.inf and all(torch.equal(a, b) for a, b in zip(before, [x for y in (p, m, v, s or []) for x in y] + [steps]))
+
+
+def test_first_step_is_not_captured(monkeypatch):
+    w = torch.nn.Parameter(torch.ones(9, device=DEV))
+    w.grad = torch.ones_like(w)
+    opt = optim.AdamW([w])
+    with monkeypatch.context() as patch:
+        patch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+        with pytest.raises(RuntimeError, match="captured"):
+            opt.step()
+    opt.step()
+    assert float(opt.state[w]["step"]) == 1
+
+
+def test_captured_step_of_the_class():
+    """A first step, the capture, replays with an eager step between them: as many eager steps."""
+    nets = [networks().to(DEV) for _ in range(2)]
+    opts = [optim.AdamW(n.parameters(), lr=1e-3, state_bits=8, min_8bit_numel=256, max_norm=1e-2) for n in nets]
+    x = torch.randn(32, 3, generator=torch.Generator().manual_seed(0)).to(DEV)
+    for net, opt in zip(nets, opts):
+        net(x).square().mean().backward()
+        opt.step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opts[0].step()                                   # records the step, runs nothing
+    for k in range(4):
+        for net in nets:
+            for p in net.parameters():
+                p.grad.mul_(1.1)
+        graph.replay() if k != 2 else opts[0].step()
+        opts[1].step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(nets[0].parameters(), nets[1].parameters())), k
 
 
 @pytest.mark.parametrize("bits", [32, 8])

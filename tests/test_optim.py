@@ -80,14 +80,16 @@ def test_step_refuses(what, change):
     ("scales of the wrong type", dict(scales=lambda x: [x[0], x[1].double()])),
     ("scales too few", dict(scales=lambda x: x[:1])),
     ("codes off their alignment", dict(exp_avgs=lambda x: [x[0], torch.zeros(513, dtype=torch.int8)[1:].view(2, 256)])),
+    ("eps below what the 8-bit step resolves", dict(eps=1e-31)),
     ("codes with gaps", dict(exp_avg_sqs=lambda x: [x[0], torch.zeros(2, 512, dtype=torch.uint8)[:, ::2]])),
 ])
 def test_8_bit_step_refuses(what, change):
-    args = lists(bits=8)
+    args = dict(lists(bits=8), eps=1e-8)
     for k, f in change.items():
-        args[k] = f(args[k])
+        args[k] = f(args[k]) if callable(f) else f
     with pytest.raises(ValueError):
-        optim.adamw8_step(*(args[k] for k in ("params", "grads", "exp_avgs", "exp_avg_sqs", "scales", "steps")), lr=1e-3)
+        optim.adamw8_step(*(args[k] for k in ("params", "grads", "exp_avgs", "exp_avg_sqs", "scales", "steps")), lr=1e-3,
+                          eps=args["eps"])
 
 
 def test_no_parameters_is_no_work():
@@ -275,6 +277,16 @@ def test_load_state_dict_refuses():
             opt.load_state_dict(bad.state_dict())
 
 
+def test_load_state_dict_refuses_other_shapes():
+    net = networks()
+    opt = optim.AdamW(net.parameters())
+    train_steps(net, opt, 1)
+    saved = opt.state_dict()
+    saved["state"][0] = {**saved["state"][0], "exp_avg": torch.zeros(1)}
+    with pytest.raises(ValueError):
+        optim.AdamW(networks().parameters()).load_state_dict(saved)
+
+
 def test_skip_nonfinite_changes_nothing():
     p, g, m, v, _, steps = U.make([300, 5], torch.float32, 32, "cpu")
     keep = [t.clone() for x in (p, m, v) for t in x]
@@ -357,6 +369,8 @@ def c_step(n=1, **change):
     (1, dict(scales=(ctypes.c_void_p * 1)(4096), m=(ctypes.c_void_p * 1)(4100))),
     (1, dict(group=(Group * 1)(Group(1e-3, 1.0, 0.99, 1e-8, 0.0, None)))),
     (1, dict(group=(Group * 1)(Group(math.nan, 0.9, 0.99, 1e-8, 0.0, None)))),
+    (1, dict(params=(ctypes.c_void_p * 1)(4098))), (1, dict(steps=(ctypes.c_void_p * 1)(4097))),
+    (1, dict(scales=(ctypes.c_void_p * 1)(4096), group=(Group * 1)(Group(1e-3, 0.9, 0.99, 1e-31, 0.0, None)))),
     (3, dict(size=16)), (3, dict(work=None, size=1 << 20)),
     (4, dict(numels=(ctypes.c_long * 1)(1 << 60))),
 ])
