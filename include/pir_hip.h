@@ -282,7 +282,7 @@ size_t pir_adamw_workspace_bytes(int n, const long* numels, int with_norm);
  * exp_avg_sqs[i] are fp32[numels[i]].  Otherwise they are 8-bit codes, int8 and uint8 [ceil(numels[i] / 256) * 256],
  * and scales[i] is fp32 [ceil(numels[i] / 256)][2]: m = s0 (q / 127) |q / 127|, v = s1 (c / 255)^4, s0 and s1 the
  * largest |m| and v of 256 consecutive elements (codes aligned to 16 bytes, scales to 8; what lies behind numels[i] is written as zero).  A
- * moment that is not finite makes its block's scales NaN; eps has to be 1e-30 at least.  groups[i]: index into group.  skip_nonfinite: if |g| is not
+ * moment that is not finite makes its block's scale NaN, a second one both scales; eps has to be 1e-30 at least.  groups[i]: index into group.  skip_nonfinite: if |g| is not
  * finite nothing changes, the step counts included.  total_norm: optional DEVICE float that receives |g|.
  * No two tensors of a call may overlap, step counts included. */
 int pir_adamw_step(int n, void* const* params, const void* const* grads, void* const* exp_avgs, void* const* exp_avg_sqs,

@@ -318,7 +318,8 @@ adamw8_kernel(const UpdateArgs args) {
   }
   const float nb = block_scale(half_max(mb));
   float na = block_scale(half_max(__float_as_uint(ma)));
-  na = nb != nb ? nb : na;                  // the maximum of floats passes over a NaN, which v has too
+  // the maximum of floats passes over a NaN: one of g is in v too, one of a scale is in the whole block
+  na = nb != nb ? nb : ab.x != ab.x ? ab.x : na;
   const float ra = na > 0.0f ? 1.0f / na : 0.0f, rb = nb > 0.0f ? __builtin_amdgcn_rsqf(nb) : 0.0f;
   const float live = nb > 0.0f ? 0x1p127f : 0.0f;
 #pragma unroll

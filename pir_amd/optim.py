@@ -17,8 +17,9 @@ With t the step count of a tensor and g its gradient, times min(1, max_norm / (|
 computed in fp32 and rounded once to p's type (fp32, bf16 or fp16; gradients have the type of their parameter).  The 8-bit
 moments of 256 consecutive elements are m = a (q / 127) |q / 127| (int8 q) and v = b (c / 255)^4 (uint8 c) with a, b the
 block's largest |m| and v in fp32, rounded to the nearest code, except that a v above zero keeps c >= 1 (in a step: a v of
-2^-126 or more).  A block whose largest is below 2^-126 is zero; one that holds an infinity or a NaN has a scale of NaN, as that element would have
-moments of NaN in 32 bits: skip_nonfinite leaves everything as it is in such a step.
+2^-126 or more).  A block whose largest is below 2^-126 is zero; one that holds an infinity or a NaN has a scale of NaN, and
+a step that finds one in v sets both scales so: what a bad gradient does to its own moments in 32 bits, it does to its
+block's in 8.  skip_nonfinite leaves everything as it is in a step whose joint norm is not finite in fp32.
 
 Step counts live on the device (fp32, one per tensor), so that a step can be captured into a HIP graph and replayed; a
 learning rate that changes between replays is a one-element fp32 device tensor.  Calls enqueue work on the current stream
@@ -219,8 +220,10 @@ def _run_torch(params, grads, exp_avgs, exp_avg_sqs, scales, steps, groups, hype
             p.copy_(w - (lr * decay * w + size * (m / (v.sqrt() / root + eps))))
             if s is not None:
                 flat = (numel,), (1,)
-                for out, new in zip((*codes, s), _encode_torch(m.as_strided(*flat), v.as_strided(*flat))):
-                    out.copy_(new)
+                new = _encode_torch(m.as_strided(*flat), v.as_strided(*flat))
+                new[2][:, 0].masked_fill_(new[2][:, 1].isnan(), math.nan)
+                for x, y in zip((*codes, s), new):
+                    x.copy_(y)
         return norm
 
 
@@ -356,7 +359,7 @@ class AdamW(torch.optim.Optimizer):
     state_bits=8 keeps the moments of parameters of at least min_8bit_numel elements in 8 bits (2.03 bytes a parameter in
     place of 8); smaller ones, biases above all, stay in 32.  max_norm clips the joint gradient norm of the optimizer's
     parameters inside the step, without a pass of its own; skip_nonfinite leaves parameters, moments and step counts as
-    they are in a step whose gradients hold an infinity or a NaN.  Either leaves the norm before clipping in total_norm, a
+    they are in a step whose joint norm is not finite.  Either leaves the norm before clipping in total_norm, a
     device tensor.  A parameter without a gradient is skipped: no state, no step counted.
 
     state[p]: "step" (fp32, on p's device), "exp_avg", "exp_avg_sq" and, in 8 bits, "scales".  load_state_dict takes the

@@ -149,6 +149,18 @@ def test_gradients_that_are_not_finite(bits):
     assert torch.equal(steps, before[-1] + 1) and not torch.equal(p[0], keep[0])
 
 
+@pytest.mark.parametrize("device", ["cpu", DEV])
+def test_scales_of_moments_that_are_not_finite(device):
+    """A second moment past fp32's largest takes both scales of its block with it; a first moment's scale that is NaN stays
+    so, and says nothing about other blocks."""
+    p, g, m, v, s, steps = U.make([1024], torch.float32, 8, device)
+    g[0][300] = 1e21                                     # 0.001 1e42
+    s[0][2, 0] = math.nan
+    run(p, g, m, v, s, steps, None, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.0)
+    assert s[0].isnan().tolist() == [[False, False], [True, True], [True, False], [False, False]]
+    assert p[0].isnan().nonzero().view(-1).tolist() == list(range(512, 768))
+
+
 def test_blocks_without_gradients_keep_their_parameters():
     """Moments of zero and gradients of zero: no step, and 0 / (0 + eps) is no NaN; a block that then gets one starts."""
     p = [torch.randn(600, device=DEV)]
