@@ -385,6 +385,38 @@ def test_two_graphs_side_by_side():
                 assert all(torch.equal(i, j) for i, j in zip(x, y))
 
 
+def test_one_optimizer_on_two_devices():
+    ps = [torch.nn.Parameter(torch.ones(300)), torch.nn.Parameter(torch.ones(300, device=DEV))]
+    opt = optim.AdamW(ps, lr=1e-2, weight_decay=0.0)
+    for p in ps:
+        p.grad = torch.full_like(p, 0.5)
+    opt.step()
+    assert all(float((1 - p.detach() - 1e-2).abs().max()) < 2e-7 for p in ps)
+    with pytest.raises(ValueError, match="several devices"):
+        optim.step_together([opt], max_norm=1.0)
+
+
+def test_c_calls_with_the_least():
+    """A norm without those of each, a norm of nothing, a step of nothing that is asked for its norm."""
+    import ctypes
+    from pir_amd import _lib
+    L, stream = _lib.lib(), torch.cuda.current_stream().cuda_stream
+    g = torch.full((10_000,), 2.0, device=DEV)
+    out, work = torch.full((3,), -1.0, device=DEV), torch.empty(1 << 16, dtype=torch.uint8, device=DEV)
+    grads, numels, dtypes = (ctypes.c_void_p * 1)(g.data_ptr()), (ctypes.c_long * 1)(10_000), (ctypes.c_int * 1)(0)
+    at = [ctypes.addressof(x) for x in (grads, numels, dtypes)]
+    assert L.pir_grad_norm(1, *at, out.data_ptr(), None, work.data_ptr(), work.numel(), stream) == 0
+    assert L.pir_grad_norm(0, *at, out.data_ptr() + 4, None, work.data_ptr(), work.numel(), stream) == 0
+    assert L.pir_adamw_step(0, *[None] * 10, 0, 0.0, 0, out.data_ptr() + 8, work.data_ptr(), work.numel(), stream) == 0
+    assert out.tolist() == [200.0, 0.0, 0.0]
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_empty_tensors_alone(bits):
+    U.check_step(run, [0], torch.float32, bits, DEV)
+    U.check_step(run, [0, 0, 300, 0], torch.bfloat16, bits, DEV, max_norm=1.0)
+
+
 def test_another_stream():
     p, g, m, v, s, steps = U.make([300_000], torch.float32, 32, DEV)
     q = [t.clone() for t in p], g, [t.clone() for t in m], [t.clone() for t in v], None, steps.clone()
