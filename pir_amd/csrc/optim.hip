@@ -23,8 +23,8 @@ constexpr int kPrepRows = 104;                // tensors and hyper-parameter set
 constexpr int kPrepGroups = 8;                // arguments hold
 constexpr int kPrepThreads = 1024;
 constexpr long kNormChunk = 4096;             // the smallest number of elements a workgroup sums
-constexpr int kNormTable = 160;               // tensors per launch of the norm's first pass
-constexpr int kFinishWaves = 4;               // tensors per workgroup of the norm's second pass
+constexpr int kNormTable = 312;               // tensors per launch of the norm's first pass
+constexpr int kFinishWaves = 4;              // tensors per workgroup of the second pass (16: 3.6 us, 4: 2.8 for 126 tensors)
 constexpr int kFirstTable = 1000;             // tensors per launch of that
 
 // what one tensor's update needs, computed once per step by the prologue
@@ -78,9 +78,11 @@ struct NormTable {
   int n;
   unsigned chunk;                             // elements one workgroup sums
   double* partial;
-  const void* grad[kNormTable];
-  long numel[kNormTable];                     // dtype in the lowest two bits
-  unsigned first[kNormTable];
+  const void* base;                           // the first tensor; the others by their differences, in units of 2 bytes
+  int grad[kNormTable];
+  unsigned numel[kNormTable];                 // lower 32 bits
+  unsigned first[kNormTable];                 // first workgroup
+  unsigned char more[kNormTable];             // type (2 bits), upper bits of numel
 };
 
 struct FinishTable {
@@ -256,7 +258,7 @@ __device__ inline unsigned pack_low_bytes(float a, float b, float c, float d) {
 // 8-bit moments: half a wave per block of 256 elements, 8 consecutive ones per lane.  10 bytes an element (16-bit
 // parameters) leave the vector unit about 60 operations each, so the arithmetic is counted: square roots and reciprocals
 // are the hardware's (one ulp), the root of v serves the step and the new code, codes are rounded and packed as bits, and
-// maxima cross lanes without shared memory.  435 M bf16 elements: 0.68 ms, 6.5 TB/s, bound by memory; with IEEE roots and
+// maxima cross lanes without shared memory.  435 M bf16 elements: 0.69 ms, 6.4 TB/s, bound by memory; with IEEE roots and
 // divisions and shuffles through shared memory 1.51 ms.
 template <typename T, bool kStream>
 __global__ void __launch_bounds__(kOptThreads)
@@ -440,13 +442,14 @@ __global__ void __launch_bounds__(kThreads)
 norm_partial_kernel(const NormTable tab) {
   __shared__ double part[kThreads / 64];
   const int k = find_tensor(tab.first, tab.n, blockIdx.x);
-  const long base = (long)(blockIdx.x - tab.first[k]) * tab.chunk, numel = tab.numel[k] >> 2;
+  const int dtype = tab.more[k] & 3;
+  const void* grad = (const short*)tab.base + tab.grad[k];
+  const long base = (long)(blockIdx.x - tab.first[k]) * tab.chunk, numel = (long)(tab.more[k] >> 2) << 32 | tab.numel[k];
   const long end = base + tab.chunk < numel ? base + tab.chunk : numel;
-  const int dtype = tab.numel[k] & 3;
   double s;
-  if (dtype == PIR_F32) s = sum_squares<kThreads, kStream>((const float*)tab.grad[k], base, end);
-  else if (dtype == PIR_BF16) s = sum_squares<kThreads, kStream>((const __bf16*)tab.grad[k], base, end);
-  else s = sum_squares<kThreads, kStream>((const _Float16*)tab.grad[k], base, end);
+  if (dtype == PIR_F32) s = sum_squares<kThreads, kStream>((const float*)grad, base, end);
+  else if (dtype == PIR_BF16) s = sum_squares<kThreads, kStream>((const __bf16*)grad, base, end);
+  else s = sum_squares<kThreads, kStream>((const _Float16*)grad, base, end);
   s = wave_sum(s);
   if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = s;
   __syncthreads();
@@ -470,7 +473,7 @@ __device__ inline double sum_partials(const double* __restrict__ partial, int n,
 // One workgroup: the joint norm and clip factor from the partial sums, then the step counts and coefficients of its
 // tensors (in 64 bits: 1 - beta2^t at t = 1 loses three digits in 32), and their descriptors for the update kernels.  2.4 to
 // 4 us, nearly all of it the launch and one chain of dependent reads; it spares every workgroup of the update the 64-bit
-// exponentials, and a step of many tensors all but one update launch (301 tensors: 155 us with 64 tensors a launch, 49 so).
+// exponentials, and a step of many tensors all but one update launch (301 tensors, clipped: 155 us with 64 tensors a launch, 48 so).
 __global__ void __launch_bounds__(kPrepThreads)
 adamw_prologue_kernel(const PrepTable tab) {
   __shared__ double part[kPrepThreads / 64];
@@ -587,6 +590,13 @@ static long norm_partials(int n, const long* numels) {
   return c;
 }
 
+// to - from in units of 1 << shift bytes; whether it fits
+static inline bool difference(const void* to, const void* from, int shift, int& d) {
+  const long x = ((long)to - (long)from) >> shift;
+  d = (int)x;
+  return x == d;
+}
+
 static int launch_partials(int n, const void* const* grads, const long* numels, const int* dtypes, double* partial,
                            hipStream_t stream) {
   NormTable tab;
@@ -597,18 +607,22 @@ static int launch_partials(int n, const void* const* grads, const long* numels, 
   for (int i = 0; i < n; ++i) bytes += numels[i] * element_bytes(dtypes[i]);
   for (int i = 0; i <= n; ++i) {
     const long blocks = i < n ? ceil_div(numels[i], tab.chunk) : 0;
-    if (tab.n > 0 && (i == n || tab.n == kNormTable)) {
+    if (i < n && blocks == 0) continue;
+    int away = 0;
+    if (tab.n > 0 && (i == n || tab.n == kNormTable || !difference(grads[i], tab.base, 1, away))) {
       const dim3 grid((unsigned)at);
       if (bytes > kCacheBytes) hipLaunchKernelGGL((norm_partial_kernel<1024, true>), grid, dim3(1024), 0, stream, tab);
       else if (tab.chunk > kNormChunk) hipLaunchKernelGGL((norm_partial_kernel<1024, false>), grid, dim3(1024), 0, stream, tab);
       else hipLaunchKernelGGL((norm_partial_kernel<256, false>), grid, dim3(256), 0, stream, tab);
       tab.partial += at;
       tab.n = 0;
-      at = 0;
+      at = away = 0;
     }
-    if (blocks == 0) continue;
-    tab.grad[tab.n] = grads[i];
-    tab.numel[tab.n] = numels[i] << 2 | dtypes[i];
+    if (i == n) break;
+    if (tab.n == 0) tab.base = grads[i];
+    tab.grad[tab.n] = away;
+    tab.numel[tab.n] = (unsigned)numels[i];
+    tab.more[tab.n] = (unsigned char)(numels[i] >> 32 << 2 | dtypes[i]);
     tab.first[tab.n] = (unsigned)at;
     at += blocks;
     ++tab.n;
@@ -643,13 +657,6 @@ static PrepGroup prologue_group(const PirAdamwGroup& g) {
   d.eps = (float)g.eps;
   d.pad = 0.0f;
   return d;
-}
-
-// to - from in units of 1 << shift bytes; whether it fits
-static inline bool difference(const void* to, const void* from, int shift, int& d) {
-  const long x = ((long)to - (long)from) >> shift;
-  d = (int)x;
-  return x == d;
 }
 
 // the row's addresses as differences from the launch's; false: some do not fit.  An empty tensor has none that count, and

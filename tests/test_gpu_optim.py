@@ -192,7 +192,7 @@ def test_grad_norm(dtype):
     assert torch.equal(total, again[0]) and torch.equal(each, again[1])
 
 
-@pytest.mark.parametrize("count", [1, 64, 65, 511, 512, 513, 1100])
+@pytest.mark.parametrize("count", [1, 64, 65, 312, 313, 511, 512, 513, 1100])
 def test_grad_norm_of_many(count):
     g = [torch.full((1 + i % 5,), float(i), device=DEV) for i in range(count)]
     total, each = optim.grad_norm(g)
@@ -267,10 +267,13 @@ def test_tensors_far_apart(bits):
     room = torch.empty(20 * 2 ** 30, dtype=torch.uint8, device=DEV).view(torch.float32)
     hyper = dict(lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.1)
     p, g, m, v, s, steps = U.make([5000] * 4, torch.float32, bits, DEV)
+    away = [room[i + 10_000:i + 15_000].copy_(x) for i, x in zip((0, room.numel() - 25_000, 5000, room.numel() // 2), g)]
+    for x, y in zip(optim.grad_norm(away), optim.grad_norm(g)):
+        assert torch.equal(x, y)
     near = [t.clone() for t in p], g, [t.clone() for t in m], [t.clone() for t in v], None if s is None else [t.clone() for t in s], steps.clone()
     at = [room.numel() - 5000, 0, room.numel() // 2, 5000]
     far = [room[i:i + 5000].copy_(t) for i, t in zip(at, p)]
-    run(far, g, m, v, s, steps, 0.1, **hyper)
+    run(far, away, m, v, s, steps, 0.1, **hyper)
     run(*near, 0.1, **hyper)
     assert all(torch.equal(a, b) for a, b in zip(far, near[0])) and torch.equal(steps, near[5])
     assert all(torch.equal(a, b) for a, b in zip(m, near[2])) and all(torch.equal(a, b) for a, b in zip(v, near[3]))
