@@ -463,7 +463,7 @@ def step_together(optimizers, max_norm=None, skip_nonfinite=False):
     """One step of several AdamW optimizers in one call, their gradients clipped to one joint norm.  (The optimizers' own
     max_norm and skip_nonfinite are for their own step().)  Returns the joint norm with max_norm or skip_nonfinite."""
     bound = _max_norm(max_norm)
-    jobs = {}                    # device -> its tensors, of all optimizers
+    parts = []                   # the tensors of one group on one device
     for opt in optimizers:
         if not isinstance(opt, AdamW):
             raise TypeError(f"step_together takes pir_amd.optim.AdamW optimizers, not {type(opt).__name__}")
@@ -471,14 +471,16 @@ def step_together(optimizers, max_norm=None, skip_nonfinite=False):
             live = [p for p in group["params"] if p.grad is not None]
             places = {p.get_device() for p in live}
             for place in places:
-                mine = live if len(places) == 1 else [p for p in live if p.get_device() == place]
-                states = [opt.state[p] for p in mine]
-                if not all(states):
-                    states = [opt._state_of(p, group) for p in mine]
-                job = jobs.setdefault(place, _Job(mine[0].device))
-                job.add(mine, states, _hyper(group["lr"], group["betas"], group["eps"], group["weight_decay"], job.device))
-    if len(jobs) > 1 and (bound or skip_nonfinite):
+                parts.append((place, opt, group, live if len(places) == 1 else [p for p in live if p.get_device() == place]))
+    if (max_norm is not None or skip_nonfinite) and len({place for place, *_ in parts}) > 1:
         raise ValueError("a joint norm of parameters on several devices is not supported")
+    jobs = {}                    # device -> its tensors, of all optimizers
+    for place, opt, group, mine in parts:
+        states = [opt.state[p] for p in mine]
+        if not all(states):
+            states = [opt._state_of(p, group) for p in mine]
+        job = jobs.setdefault(place, _Job(mine[0].device))
+        job.add(mine, states, _hyper(group["lr"], group["betas"], group["eps"], group["weight_decay"], job.device))
     norm = torch.zeros(()) if max_norm is not None or skip_nonfinite else None      # what no gradients have
     for job in jobs.values():
         norm = job.run(bound, skip_nonfinite, max_norm is not None)

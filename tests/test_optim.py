@@ -389,3 +389,25 @@ def test_c_calls_without_work():
     assert L.pir_moments8_encode(0, 0, None, None, None, None, None, None) == 0
     assert L.pir_moments8_encode(5, 7, None, None, None, None, None, None) == 1
     assert L.pir_grad_norm(1, None, None, None, None, None, None, 0, None) == 1
+
+
+class Elsewhere(torch.nn.Parameter):
+    """A parameter that says it lives on another device."""
+
+    def get_device(self):
+        return 7
+
+
+@pytest.mark.parametrize("ask", [dict(max_norm=1.0), dict(max_norm=math.inf), dict(skip_nonfinite=True)])
+def test_a_joint_norm_over_devices_is_refused(ask):
+    """Whatever it is for, clipping, skipping or being looked at; and before anything has a state."""
+    ps = [torch.nn.Parameter(torch.ones(9)), Elsewhere(torch.ones(16))]
+    for p in ps:
+        p.grad = torch.ones(p.shape)
+    opt = optim.AdamW(ps, **ask)
+    with pytest.raises(ValueError, match="several devices"):
+        opt.step()
+    with pytest.raises(ValueError, match="several devices"):
+        optim.step_together([opt], **ask)
+    assert len(opt.state) == 0 and all(torch.equal(p, torch.ones(p.shape)) for p in ps)
+    assert optim.step_together([opt]) is None and all(float(opt.state[p]["step"]) == 1 for p in ps)
