@@ -66,29 +66,89 @@ bool coded(const at::Tensor& q, const at::Tensor& c, const at::Tensor& s, long n
          !((size_t)address(s) & 7);
 }
 
-// whether no byte belongs to two of the tensors; most lists are in the order of memory already
-bool disjoint(const std::vector<void*>& at, const std::vector<long>& bytes, std::vector<std::pair<char*, long>>& scratch) {
-  const size_t n = at.size();
-  char* end = nullptr;
-  size_t i = 0;
-  for (; i < n; ++i) {
-    if (bytes[i] == 0) continue;
-    if ((char*)at[i] < end) break;
-    end = (char*)at[i] + bytes[i];
+// The memory of a step's tensors, in lists that are written (parameters, both moments, scales, step counts) or only read
+// (gradients).  No byte that is written may belong to two tensors; those that are only read may share theirs.
+class Memory {
+  static constexpr size_t kWritten = (size_t)1 << 63;
+  struct Span {
+    size_t at, end;                              // kWritten in end
+  };
+  struct List {
+    Span *from, *to;
+    bool ascending, written;
+    size_t lo, hi;
+  };
+  std::vector<Span> spans;
+  std::vector<List> lists;
+
+  static Span* merge(const Span* a, const Span* a_end, const Span* b, const Span* b_end, Span* out) {
+    while (a != a_end && b != b_end) {           // without a branch on which comes first: lists lie among each other
+      const bool second = b->at < a->at;
+      *out++ = second ? *b : *a;
+      b += second;
+      a += !second;
+    }
+    out = std::copy(a, a_end, out);
+    return std::copy(b, b_end, out);
   }
-  if (i == n) return true;
-  scratch.clear();
-  for (i = 0; i < n; ++i)
-    if (bytes[i]) scratch.emplace_back((char*)at[i], bytes[i]);
-  std::sort(scratch.begin(), scratch.end());
-  for (i = 1; i < scratch.size(); ++i)
-    if (scratch[i].first < scratch[i - 1].first + scratch[i - 1].second) return false;
-  return true;
-}
+
+ public:
+  enum { kParams, kGrads, kFirst, kSecond, kScales, kSteps, kLists };
+
+  explicit Memory(Py_ssize_t n) : spans(kLists * n), lists(kLists) {
+    for (int i = 0; i < kLists; ++i) lists[i] = {&spans[i * n], &spans[i * n], true, i != kGrads, ~(size_t)0, 0};
+  }
+
+  void add(int list, const void* at, long bytes) {
+    if (!bytes) return;
+    List& l = lists[list];
+    const size_t start = (size_t)at, end = start + (size_t)bytes;
+    l.ascending &= start >= l.hi;
+    l.lo = std::min(l.lo, start);
+    l.hi = std::max(l.hi, end);
+    *l.to++ = {start, l.written ? end | kWritten : end};
+  }
+
+  // Lists that are in the order of memory and apart from all others (views of a buffer each) need no more than their
+  // ends.  Others, as a model's parameters and their states lie, are merged in that order: 7 us for 500 tensors.
+  bool disjoint() {
+    std::vector<std::pair<Span*, Span*>> runs;
+    for (const List& l : lists) {
+      bool among = l.written && !l.ascending;
+      for (const List& o : lists) among |= &o != &l && l.lo < o.hi && o.lo < l.hi;
+      if (!among) continue;
+      if (!l.ascending) std::sort(l.from, l.to, [](const Span& x, const Span& y) { return x.at < y.at; });
+      runs.emplace_back(l.from, l.to);
+    }
+    if (runs.empty()) return true;
+    std::vector<Span> other(spans.size());
+    Span* to = other.data();
+    while (runs.size() > 1) {                    // pairs of runs, from one buffer to the other and back
+      Span* out = to;
+      size_t k = 0;
+      for (size_t i = 0; i < runs.size(); i += 2) {
+        const auto a = runs[i], b = i + 1 < runs.size() ? runs[i + 1] : std::make_pair(a.second, a.second);
+        Span* const end = merge(a.first, a.second, b.first, b.second, out);
+        runs[k++] = {out, end};
+        out = end;
+      }
+      runs.resize(k);
+      to = to == other.data() ? spans.data() : other.data();
+    }
+    size_t written = 0, read = 0;                // where what came so far ends
+    for (const Span* s = runs[0].first; s != runs[0].second; ++s) {
+      const bool w = s->end & kWritten;
+      if (s->at < written || (w && s->at < read)) return false;
+      size_t& end = w ? written : read;
+      end = std::max(end, s->end & ~kWritten);
+    }
+    return true;
+  }
+};
 
 struct Lists {
   std::vector<void*> p, g, m, v, s, t;
-  std::vector<long> numels, bytes, mbytes, vbytes;
+  std::vector<long> numels;
   std::vector<int> dtypes;
 };
 
@@ -114,8 +174,9 @@ PyObject* step(PyObject*, PyObject* args) {
     if (n < 1 || G.n != n || M.n != n || V.n != n || (ss != Py_None && S.n != n)) Py_RETURN_NOTIMPLEMENTED;
     Lists a;
     for (auto* x : {&a.p, &a.g, &a.m, &a.v, &a.s, &a.t}) x->resize(n);
-    for (auto* x : {&a.numels, &a.bytes, &a.mbytes, &a.vbytes}) x->resize(n);
+    a.numels.resize(n);
     a.dtypes.resize(n);
+    Memory memory(n);
     for (Py_ssize_t i = 0; i < n; ++i) {
       const at::Tensor *p = tensor_of(P.at[i], dev), *g = tensor_of(G.at[i], dev), *m = tensor_of(M.at[i], dev),
                        *v = tensor_of(V.at[i], dev);
@@ -125,19 +186,21 @@ PyObject* step(PyObject*, PyObject* args) {
       if (type < 0 || g->scalar_type() != p->scalar_type() || !dense(*p) || !same_layout(*p, *g)) Py_RETURN_NOTIMPLEMENTED;
       if (((size_t)address(*p) | (size_t)address(*g)) & (p->element_size() - 1)) Py_RETURN_NOTIMPLEMENTED;
       char *am = address(*m), *av = address(*v), *as = nullptr;
-      if (numel && (am == av || am == address(*p) || av == address(*p))) Py_RETURN_NOTIMPLEMENTED;
       PyObject* so = ss == Py_None ? Py_None : S.at[i];
       if (so == Py_None) {
         if (m->scalar_type() != at::kFloat || v->scalar_type() != at::kFloat || !same_layout(*p, *m) || !same_layout(*p, *v))
           Py_RETURN_NOTIMPLEMENTED;
-        a.mbytes[i] = a.vbytes[i] = 4 * numel;
+        memory.add(Memory::kFirst, am, 4 * numel);
+        memory.add(Memory::kSecond, av, 4 * numel);
       } else {
         const at::Tensor* s = tensor_of(so, dev);
         const long nb = (numel + 255) / 256;
         if (!s || !coded(*m, *v, *s, nb)) Py_RETURN_NOTIMPLEMENTED;
         as = address(*s);
         if (!as) as = (char*)16;                 // no blocks: 8-bit all the same
-        a.mbytes[i] = a.vbytes[i] = 256 * nb;
+        memory.add(Memory::kFirst, am, 256 * nb);
+        memory.add(Memory::kSecond, av, 256 * nb);
+        memory.add(Memory::kScales, as, 8 * nb);
       }
       a.p[i] = address(*p);
       a.g[i] = address(*g);
@@ -145,7 +208,8 @@ PyObject* step(PyObject*, PyObject* args) {
       a.v[i] = av;
       a.s[i] = as;
       a.numels[i] = numel;
-      a.bytes[i] = numel * (long)p->element_size();
+      memory.add(Memory::kParams, a.p[i], numel * (long)p->element_size());
+      memory.add(Memory::kGrads, a.g[i], numel * (long)p->element_size());
       a.dtypes[i] = type;
     }
     if (T.n >= 0) {
@@ -154,15 +218,15 @@ PyObject* step(PyObject*, PyObject* args) {
         const at::Tensor* t = tensor_of(T.at[i], dev);
         if (!t || t->scalar_type() != at::kFloat || t->numel() != 1) Py_RETURN_NOTIMPLEMENTED;
         a.t[i] = address(*t);
+        memory.add(Memory::kSteps, a.t[i], 4);
       }
     } else {
       const at::Tensor* t = tensor_of(ts, dev);
       if (!t || t->scalar_type() != at::kFloat || t->numel() != n || !t->is_contiguous()) Py_RETURN_NOTIMPLEMENTED;
       for (Py_ssize_t i = 0; i < n; ++i) a.t[i] = address(*t) + 4 * i;
+      memory.add(Memory::kSteps, a.t[0], 4 * n);
     }
-    std::vector<std::pair<char*, long>> scratch;
-    if (!disjoint(a.p, a.bytes, scratch) || !disjoint(a.m, a.mbytes, scratch) || !disjoint(a.v, a.vbytes, scratch))
-      Py_RETURN_NOTIMPLEMENTED;
+    if (!memory.disjoint()) Py_RETURN_NOTIMPLEMENTED;
     std::vector<PirAdamwGroup> table(PyList_GET_SIZE(hypers));
     for (size_t k = 0; k < table.size(); ++k) {
       unsigned long long lr = 0;

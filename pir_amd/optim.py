@@ -85,21 +85,18 @@ def _blocks(numel):
     return -(-numel // BLOCK)
 
 
-def _check_disjoint(what, tensors):
-    """Kernels write these tensors side by side: no byte may belong to two of them."""
-    at = [(t.data_ptr(), t.numel() * t.element_size()) for t in tensors]
-    end = 0
-    for start, size in at:
-        if start < end:
-            break
-        end = start + size
-    else:
-        return
-    end = 0
-    for start, size in sorted(x for x in at if x[1]):
-        if start < end:
-            raise ValueError(f"{what}: a tensor is given twice, or two of them overlap")
-        end = start + size
+def _check_disjoint(written, read):
+    """Kernels write these tensors side by side: no byte of one may belong to another of them, or to one that is read."""
+    spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size(), w)
+                   for w, tensors in ((True, written), (False, read)) for t in tensors if t.numel())
+    written_to = read_to = 0
+    for start, end, w in spans:
+        if start < written_to or (w and start < read_to):
+            raise ValueError("tensors that the step writes: one is given twice, or overlaps another or a gradient")
+        if w:
+            written_to = max(written_to, end)
+        else:
+            read_to = max(read_to, end)
 
 
 def _same_layout(p, t):
@@ -111,8 +108,8 @@ def _check_eps(eps, coded):
         raise ValueError(f"eps: at least {_LEAST_EPS} with 8-bit moments, not {eps}")
 
 
-def _check(params, grads, exp_avgs, exp_avg_sqs, scales):
-    """Checks the lists of one device; gradients that are laid out unlike their parameters come back as copies."""
+def _check(params, grads, exp_avgs, exp_avg_sqs, scales, steps):
+    """Checks the lists of one device (steps: a tensor or a list of them); gradients that are laid out unlike their parameters come back as copies."""
     n = len(params)
     if not len(grads) == len(exp_avgs) == len(exp_avg_sqs) == n or (scales is not None and len(scales) != n):
         raise ValueError("params, grads and moments: lists of one length")
@@ -129,8 +126,6 @@ def _check(params, grads, exp_avgs, exp_avg_sqs, scales):
             raise ValueError(f"tensors {i}: their addresses are not multiples of their type's size")
         if not p.is_contiguous() and not _dense(p):
             raise ValueError(f"parameter {i}: its elements do not fill one stretch of memory (strides {p.stride()})")
-        if p.numel() and len({p.data_ptr(), m.data_ptr(), v.data_ptr()}) < 3:
-            raise ValueError(f"tensors {i}: one of them is given twice")
         s = scales[i] if scales is not None else None
         if s is None:
             if m.dtype != torch.float32 or v.dtype != torch.float32 or not (_same_layout(p, m) and _same_layout(p, v)):
@@ -146,9 +141,8 @@ def _check(params, grads, exp_avgs, exp_avg_sqs, scales):
         if g.is_neg() or not _same_layout(p, g):
             g = torch.empty_like(p, requires_grad=False).copy_(g)
         out.append(g)
-    _check_disjoint("params", params)
-    _check_disjoint("first moments", exp_avgs)
-    _check_disjoint("second moments", exp_avg_sqs)
+    _check_disjoint([*params, *exp_avgs, *exp_avg_sqs, *(s for s in scales or () if s is not None),
+                     *([steps] if isinstance(steps, torch.Tensor) else steps)], out)
     return out
 
 
@@ -184,7 +178,7 @@ def _run(params, grads, exp_avgs, exp_avg_sqs, scales, steps, groups, hypers, ma
             skip_nonfinite, want_norm, dev.index, _stream(dev))
     norm = host.adamw_step(step, size, params, grads, *rest)
     if norm is NotImplemented:
-        grads = _check(params, grads, exp_avgs, exp_avg_sqs, scales)
+        grads = _check(params, grads, exp_avgs, exp_avg_sqs, scales, steps)
         norm = host.adamw_step(step, size, params, grads, *rest)
         if norm is NotImplemented:
             raise ValueError("plain tensors of one device are wanted")
@@ -243,7 +237,7 @@ def _step(params, grads, exp_avgs, exp_avg_sqs, scales, steps, lr, betas, eps, w
     if hyper[5] and dev.type != "cuda":
         raise ValueError("lr: on another device than the parameters")
     if dev.type != "cuda":
-        grads = _check(params, grads, exp_avgs, exp_avg_sqs, scales)
+        grads = _check(params, grads, exp_avgs, exp_avg_sqs, scales, steps)
         return _run_torch(params, grads, exp_avgs, exp_avg_sqs, scales, list(steps.view(-1)), [0] * len(params), [hyper],
                           bound, skip_nonfinite, want)
     return _run(params, grads, list(exp_avgs), list(exp_avg_sqs), scales, steps, None, [hyper], bound, skip_nonfinite, want)
@@ -252,8 +246,9 @@ def _step(params, grads, exp_avgs, exp_avg_sqs, scales, steps, lr, betas, eps, w
 def adamw_step(params, grads, exp_avgs, exp_avg_sqs, steps, *, lr, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.0,
                max_norm=None, skip_nonfinite=False):
     """One AdamW step, in place, of lists of tensors on one device; moments are fp32 with their parameter's shape and
-    strides, steps is fp32 [len(params)], all of it zero before the first step.  Returns the joint gradient norm (before
-    clipping; a 0-dim device tensor) with max_norm (inf: not clipped) or skip_nonfinite, else None."""
+    strides, steps is fp32 [len(params)], all of it zero before the first step.  None of what the step writes may share
+    memory with another tensor of the call.  Returns the joint gradient norm (before clipping; a 0-dim device tensor) with
+    max_norm (inf: not clipped) or skip_nonfinite, else None."""
     return _step(params, grads, exp_avgs, exp_avg_sqs, None, steps, lr, betas, eps, weight_decay, max_norm, skip_nonfinite)
 
 
@@ -496,7 +491,8 @@ class _Job:
     def add(self, params, states, hyper):
         if hyper[5] and self.device.type != "cuda":
             raise ValueError("lr: on another device than the parameters")
-        _check_eps(hyper[3], any("scales" in s for s in states))
+        if hyper[3] < _LEAST_EPS:
+            _check_eps(hyper[3], any("scales" in s for s in states))
         self.params += params
         self.states += states
         self.groups.extend([len(self.hypers)] * len(params))
@@ -509,4 +505,4 @@ class _Job:
         rest = (t, self.groups, self.hypers, bound, skip_nonfinite, want_norm)
         if self.device.type == "cuda":
             return _run(self.params, grads, m, v, scales, *rest)
-        return _run_torch(self.params, _check(self.params, grads, m, v, scales), m, v, scales, *rest)
+        return _run_torch(self.params, _check(self.params, grads, m, v, scales, t), m, v, scales, *rest)

@@ -8,7 +8,7 @@ import torch
 
 import optim_util as U
 from pir_amd import optim, train
-from test_optim import assert_moved_alike, networks, run, train_steps
+from test_optim import assert_moved_alike, networks, overlaps, refused_call, run, train_steps
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -565,3 +565,40 @@ def test_training_step_clips_the_joint_norm():
         bound = 6 * U.E * 0.1 * p.grad.double().abs() * 1e-3 / want + 1e-44
         assert bool(((opt.state[p]["exp_avg"] - 0.1 * p.grad.double() * min(1.0, 1e-3 / (want + 1e-6))).abs() <= bound).all())
         assert not torch.equal(p, q)
+
+
+@pytest.mark.parametrize("bits, what", [(b, w) for b in (32, 8) for w in overlaps(b)])
+def test_overlapping_tensors_are_refused(bits, what):
+    refused_call(bits, what, DEV)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_tensors_in_any_order_of_memory(bits):
+    """Lists whose tensors lie among each other in one buffer, backwards, gradients shared: what the same values give in
+    tensors of their own."""
+    n, k = 1024, 12
+    gen = torch.Generator().manual_seed(2)
+    values = torch.randn(2, k, n, generator=gen).to(DEV)
+    room = torch.empty(2 * k * n, device=DEV).view(k, 2, n)
+    p = [room[k - 1 - i, i % 2] for i in range(k)]
+    m = [room[k - 1 - i, 1 - i % 2] for i in range(k)]
+    g = [values[0, i // 2] for i in range(k)]
+    for x, y in zip(p, values[1]):
+        x.copy_(y)
+    own = [y.clone() for y in values[1]]
+    zero = lambda: [torch.zeros(n, device=DEV) for _ in range(k)]  # noqa: E731
+    if bits == 32:
+        for x in m:
+            x.zero_()
+        mine, theirs = (m, zero(), None), (zero(), zero(), None)
+    else:                                                # codes and scales in what the moments would take
+        q = [x.view(torch.int8)[:n].view(4, 256).zero_() for x in m]
+        c = [x.view(torch.uint8)[n:2 * n].view(4, 256).zero_() for x in m]
+        s = [x[512:520].view(4, 2).zero_() for x in m]
+        mine, theirs = (q, c, s), tuple(map(list, zip(*(optim.moments8_encode(x, x) for x in zero()))))
+    hyper = dict(lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.1)
+    for _ in range(2):
+        run(p, g, *mine, torch.zeros(k, device=DEV), 0.5, **hyper)
+        run(own, [x.clone() for x in g], *theirs, torch.zeros(k, device=DEV), 0.5, **hyper)
+    assert all(torch.equal(x, y) for x, y in zip(p, own))
+    assert all(torch.equal(x, y) for a, b in zip(mine, theirs) if a is not None for x, y in zip(a, b))

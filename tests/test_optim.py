@@ -411,3 +411,62 @@ def test_a_joint_norm_over_devices_is_refused(ask):
         optim.step_together([opt], **ask)
     assert len(opt.state) == 0 and all(torch.equal(p, torch.ones(p.shape)) for p in ps)
     assert optim.step_together([opt]) is None and all(float(opt.state[p]["step"]) == 1 for p in ps)
+
+
+def overlaps(bits):
+    """What one call may not be given: two of the tensors it writes, or one of those and a gradient, share memory."""
+    cases = {
+        "moments crossed": lambda a: a.update(exp_avg_sqs=a["exp_avgs"][::-1]) if bits == 32 else
+        a.update(exp_avg_sqs=[t.view(torch.uint8) for t in a["exp_avgs"][::-1]]),
+        "a step count twice": lambda a: a.update(steps=[a["steps"][:1].view(()), a["steps"][:1].view(())]),
+        "step counts in a parameter": lambda a: a.update(steps=a["params"][1][10:12]),
+        "a gradient that is a parameter": lambda a: a.update(grads=a["params"]),
+        "a gradient that starts inside a parameter": lambda a: a.update(grads=[a["grads"][0], a["room"][100:400]],
+                                                                        params=[a["params"][0], a["room"][:300]]),
+    }
+    if bits == 32:
+        cases["a parameter that ends inside a moment"] = lambda a: a.update(params=[a["params"][0], a["room"][:300]],
+                                                                            exp_avgs=[a["room"][299:599], a["exp_avgs"][1]])
+        cases["a gradient that is another's moment"] = lambda a: a.update(grads=[a["exp_avg_sqs"][1], a["grads"][1]])
+    else:
+        cases["scales twice"] = lambda a: a.update(scales=[a["scales"][0]] * 2)
+        cases["scales that overlap"] = lambda a: a.update(scales=[a["room"][:4].view(2, 2), a["room"][2:6].view(2, 2)])
+        cases["scales in a parameter"] = lambda a: a.update(scales=[a["scales"][0], a["params"][0][100:104].view(2, 2)])
+    return cases
+
+
+def refused_call(bits, what, device="cpu"):
+    """Makes one of those calls, through the list call or, for lists of step counts, as the class makes it; nothing of what
+    it was given may have moved."""
+    args = {k: [t.to(device) for t in v] if isinstance(v, list) else v.to(device) for k, v in lists(bits=bits).items()}
+    args["room"] = torch.zeros(600, device=device)
+    overlaps(bits)[what](args)
+    del args["room"]
+    given = [t for v in args.values() for t in v]        # the very tensors of the call, its step counts among them
+    before = [t.clone() for t in given]
+    with pytest.raises(ValueError, match="overlap"):
+        if isinstance(args["steps"], list):
+            from array import array
+            run_list = optim._run if device == "cuda" else optim._run_torch
+            grads = args["grads"] if device == "cuda" else optim._check(*(args.get(k) for k in (
+                "params", "grads", "exp_avgs", "exp_avg_sqs", "scales", "steps")))
+            run_list(args["params"], grads, args["exp_avgs"], args["exp_avg_sqs"], args.get("scales"), args["steps"],
+                     array("i", [0, 0]), [(1e-3, 0.9, 0.999, 1e-8, 0.0, 0)], 0.0, False, False)
+        else:
+            (optim.adamw8_step if bits == 8 else optim.adamw_step)(*[args[k] for k in (
+                "params", "grads", "exp_avgs", "exp_avg_sqs", "scales", "steps") if k in args], lr=1e-3)
+    assert all(torch.equal(a, b) for a, b in zip(given, before))
+
+
+@pytest.mark.parametrize("bits, what", [(b, w) for b in (32, 8) for w in overlaps(b)])
+def test_overlapping_tensors_are_refused(bits, what):
+    refused_call(bits, what)
+
+
+def test_one_gradient_for_two_parameters():
+    """Gradients are only read: they may share memory."""
+    g = torch.randn(300, generator=torch.Generator().manual_seed(0))
+    p = [torch.ones(300), torch.ones(300)]
+    m, v = ([torch.zeros(300), torch.zeros(300)] for _ in "mv")
+    optim.adamw_step(p, [g, g], m, v, torch.zeros(2), lr=1e-3)
+    assert torch.equal(p[0], p[1]) and torch.equal(m[0], m[1]) and not torch.equal(p[0], torch.ones(300))
