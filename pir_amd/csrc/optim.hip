@@ -208,6 +208,7 @@ __device__ inline float block_scale(unsigned top) {
 }
 
 __device__ inline unsigned umax(unsigned a, unsigned b) { return a > b ? a : b; }
+__device__ inline unsigned umin(unsigned a, unsigned b) { return a < b ? a : b; }
 __device__ inline unsigned magnitude(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 
 template <int kCtrl>
@@ -296,7 +297,7 @@ adamw8_kernel(const UpdateArgs args) {
   }
   const float a1 = c.b1 * ab.x, b2 = c.b2 * ab.y;
   float ma = 0.0f;
-  unsigned mb = 0;
+  unsigned mb = 0, low = ~0u;
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     const int qj = (int)((j < 4 ? q.x : q.y) << (24 - 8 * (j & 3))) >> 24;
@@ -304,12 +305,25 @@ adamw8_kernel(const UpdateArgs args) {
     const float x = (float)qj * (1.0f / 127.0f), y = (float)wj * (1.0f / 255.0f), y2 = y * y;
     const float gj = g[j] * c.gscale;
     m[j] = fmaf(a1, x * fabsf(x), c.c1 * gj);
-    const float v = fmaf(b2, y2 * y2, c.c2 * gj * gj);
-    r[j] = __builtin_amdgcn_sqrtf(v);
+    r[j] = fmaf(b2, y2 * y2, c.c2 * gj * gj);
+    ma = fmaxf(ma, fabsf(m[j]));
+    mb = umax(mb, __float_as_uint(r[j]));   // v is not below zero: its bits order as it does, NaN on top
+    low = umin(low, __float_as_uint(r[j]));
+  }
+  if (low < 0x00800000u) {                  // the hardware's root takes what is below 2^-126 for zero: 2^64 v, 2^-32 its root
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const bool tiny = r[j] < 0x1p-126f;
+      r[j] = __builtin_amdgcn_sqrtf(r[j] * (tiny ? 0x1p64f : 1.0f)) * (tiny ? 0x1p-32f : 1.0f);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) r[j] = __builtin_amdgcn_sqrtf(r[j]);
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
     const float u = m[j] * __builtin_amdgcn_rcpf(fmaf(r[j], c.root, c.eps));
     p[j] -= fmaf(c.decay, p[j], c.size * u);
-    ma = fmaxf(ma, fabsf(m[j]));
-    mb = umax(mb, __float_as_uint(v));      // v is not below zero: its bits order as it does, NaN on top
   }
   if (whole) {
     store<kStream>(P + i, p);

@@ -16,8 +16,9 @@ With t the step count of a tensor and g its gradient, times min(1, max_norm / (|
 
 computed in fp32 and rounded once to p's type (fp32, bf16 or fp16; gradients have the type of their parameter).  The 8-bit
 moments of 256 consecutive elements are m = a (q / 127) |q / 127| (int8 q) and v = b (c / 255)^4 (uint8 c) with a, b the
-block's largest |m| and v in fp32, rounded to the nearest code, except that a v above zero keeps c >= 1 (in a step: a v of
-2^-126 or more).  A block whose largest is below 2^-126 is zero; one that holds an infinity or a NaN has a scale of NaN, and
+block's largest |m| and v in fp32, rounded to the nearest code, except that a v above zero keeps c >= 1.  A block whose
+largest is below 2^-126 is zero (its next steps start from v = 0, up to (1 - beta2)^-1/2 times as long as in 32 bits unless
+eps is 1e-15 or more, next to which such roots are nothing); one that holds an infinity or a NaN has a scale of NaN, and
 a step that finds one in v sets both scales so: what a bad gradient does to its own moments in 32 bits, it does to its
 block's in 8.  skip_nonfinite leaves everything as it is in a step whose joint norm is not finite in fp32.
 
@@ -35,7 +36,8 @@ from . import _lib
 
 BLOCK = 256                      # elements that share a scale
 _TINY = 2.0 ** -126              # blocks whose largest is below this are zero
-_LEAST_EPS = 1e-30               # with 8-bit moments: their roots take what is below 2^-126 for zero
+_LEAST_EPS = 1e-30               # with 8-bit moments: the step's reciprocals are the hardware's, which take what is below
+                                 # 2^-126 for zero
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 

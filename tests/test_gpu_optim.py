@@ -602,3 +602,39 @@ def test_tensors_in_any_order_of_memory(bits):
         run(own, [x.clone() for x in g], *theirs, torch.zeros(k, device=DEV), 0.5, **hyper)
     assert all(torch.equal(x, y) for x, y in zip(p, own))
     assert all(torch.equal(x, y) for a, b in zip(mine, theirs) if a is not None for x, y in zip(a, b))
+
+
+@pytest.mark.parametrize("device", ["cpu", DEV])
+@pytest.mark.parametrize("eps", [1e-30, 1e-20, 1e-17, 1e-8])
+@pytest.mark.parametrize("bits", [32, 8])
+def test_second_moments_below_the_normal_numbers(bits, eps, device):
+    """First steps of gradients from 3e-20 to 1e-15: v = 0.001 g^2 goes from 9e-43, where fp32 has steps of 2^-149, to
+    1e-33.  Its one rounding to such a step is off by half of it, so a root by 2^-150 / (2 v) of itself (4e-4 at most)
+    beside the usual; twice that is allowed, since the formula's root is taken at v as it was."""
+    n = 3000
+    gen = torch.Generator().manual_seed(6)
+    g = torch.exp(torch.empty(n).uniform_(math.log(3e-20), math.log(1e-15), generator=gen)) * (torch.rand(n, generator=gen) - 0.5).sign()
+    p = 0.05 * torch.randn(n, generator=gen)
+    hyper = dict(lr=1e-3, betas=(0.9, 0.999), eps=eps, weight_decay=0.0)
+    zero = torch.zeros(n)
+    want, bound = U.step64(p, g, zero, zero, 1, **hyper)
+    update = (want[0] - p.double()).abs()
+    bound = bound[0] + update * 2.0 ** -149 / (2 * want[2].clamp(min=2.0 ** -149))
+    m, v, s = (zero.clone(), zero.clone(), None) if bits == 32 else optim.moments8_encode(zero, zero)
+    to = lambda x: [x.to(device)]  # noqa: E731
+    here = to(p.clone())
+    run(here, to(g), to(m), to(v), None if s is None else to(s), torch.zeros(1, device=device), None, **hyper)
+    U.assert_near(here[0], want[0], bound, f"eps {eps}")
+
+
+@pytest.mark.parametrize("device", ["cpu", DEV])
+def test_small_second_moments_beside_large_ones_keep_a_code(device):
+    """A v above zero has c >= 1 after a step too, however small it is: one element of each block has a gradient of 1."""
+    g = torch.full((1024,), 1e-19)                       # 0.001 g^2 = 1e-41
+    g[::256], g[5::256] = 1.0, 0.0
+    zero = torch.zeros(1024)
+    q, c, s = (x.to(device) for x in optim.moments8_encode(zero, zero))
+    optim.adamw8_step([torch.ones(1024, device=device)], [g.to(device)], [q], [c], [s], torch.zeros(1, device=device), lr=1e-3)
+    want = torch.ones(4, 256, dtype=torch.uint8)
+    want[:, 0], want[:, 5] = 255, 0
+    assert torch.equal(c.cpu(), want)
