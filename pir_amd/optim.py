@@ -420,14 +420,18 @@ class AdamW(torch.optim.Optimizer):
         return loss
 
     def load_state_dict(self, state_dict):
-        """Takes what state_dict() of this class, torch.optim.Adam or torch.optim.AdamW returns."""
+        """Takes what state_dict() of this class, torch.optim.Adam or torch.optim.AdamW returns; state_bits and min_8bit_numel
+        of the groups stay this optimizer's, and the moments are converted to them."""
         for g in state_dict["param_groups"]:
             if g.get("amsgrad") or g.get("maximize"):
                 raise ValueError("amsgrad and maximize are not supported")
             if g.get("weight_decay") and not g.get("decoupled_weight_decay", True):
                 raise ValueError("the weight decay of torch.optim.Adam (added to the gradient) is not supported")
         saved = state_dict["state"]
+        own = [{k: g[k] for k in ("state_bits", "min_8bit_numel")} for g in self.param_groups]
         super().load_state_dict({**state_dict, "state": {}})
+        for g, bits in zip(self.param_groups, own):
+            g.update(bits)
         ids = [i for g in state_dict["param_groups"] for i in g["params"]]
         for i, (p, g) in zip(ids, [(p, g) for g in self.param_groups for p in g["params"]]):
             if i in saved and saved[i]:

@@ -470,3 +470,51 @@ def test_one_gradient_for_two_parameters():
     m, v = ([torch.zeros(300), torch.zeros(300)] for _ in "mv")
     optim.adamw_step(p, [g, g], m, v, torch.zeros(2), lr=1e-3)
     assert torch.equal(p[0], p[1]) and torch.equal(m[0], m[1]) and not torch.equal(p[0], torch.ones(300))
+
+
+def assert_same_moments(a, pa, b, pb, parts):
+    """Moments of two optimizers' parameters: alike to the bit, or to parts (first, second) of their block's largest."""
+    def values(opt, p):
+        s = opt.state[p]
+        if "scales" not in s:
+            return s["exp_avg"], s["exp_avg_sq"]
+        flat = [x.reshape(-1)[:p.numel()] for x in optim.moments8_decode(s["exp_avg"], s["exp_avg_sq"], s["scales"])]
+        return [x.as_strided(p.shape, p.stride()) for x in flat]
+    for x, y, part in zip(values(a, pa), values(b, pb), parts):
+        assert float((x - y).abs().max()) <= part * float(x.abs().max())
+
+
+# the largest error of a code: at x = 1 of x^2 in steps of 1/127, and of x^4 in steps of 1/255 (the least code stands for
+# more than that only below 2.5e-10), with the rounding's own square and the fp32 evaluation
+CODE_PARTS = (1 / 127 + 1 / 254 ** 2, 2 / 255 + 6 * (0.5 / 255) ** 2 + 1e-6)
+
+
+@pytest.mark.parametrize("source", ["torch", 32, 8])
+def test_load_state_dict_keeps_the_optimizers_own_bits(source):
+    """Whatever the state comes from, each group holds it in its own number of bits, and takes the other settings."""
+    net, other = networks(), networks()
+    ours = lambda n, **k: optim.AdamW(n.parameters(), lr=3e-3, weight_decay=0.0, **k)  # noqa: E731
+    first = torch.optim.Adam(net.parameters(), lr=3e-3) if source == "torch" else ours(net, state_bits=source, min_8bit_numel=50)
+    train_steps(net, first, 3)
+    for bits, least in ((32, 4096), (8, 4096), (8, 100)):
+        second = optim.AdamW(other.parameters(), lr=1e-4, state_bits=bits, min_8bit_numel=least)
+        second.load_state_dict(first.state_dict())
+        g = second.param_groups[0]
+        assert (g["state_bits"], g["min_8bit_numel"], g["lr"], g["weight_decay"]) == (bits, least, 3e-3, 0.0)
+        for p, q in zip(net.parameters(), other.parameters()):
+            coded = bits == 8 and q.numel() >= least
+            assert ("scales" in second.state[q]) == coded and float(second.state[q]["step"]) == 3
+            moved = coded != ("scales" in first.state[p])
+            assert_same_moments(first, p, second, q, CODE_PARTS if moved else (0.0, 0.0))
+
+
+@pytest.mark.parametrize("source", ["torch", 32])
+def test_load_state_dict_into_groups_of_their_own(source):
+    net = networks()
+    halves = lambda: [{"params": list(net.parameters())[:3]}, {"params": list(net.parameters())[3:]}]  # noqa: E731
+    first = torch.optim.AdamW(halves(), lr=1e-3) if source == "torch" else optim.AdamW(halves(), lr=1e-3)
+    train_steps(net, first, 2)
+    second = optim.AdamW([{**halves()[0], "state_bits": 8, "min_8bit_numel": 1}, halves()[1]], lr=1e-4)
+    second.load_state_dict(first.state_dict())
+    assert [g["state_bits"] for g in second.param_groups] == [8, 32] and [g["lr"] for g in second.param_groups] == [1e-3, 1e-3]
+    assert ["scales" in second.state[p] for p in net.parameters()] == [True] * 3 + [False] * 3
