@@ -435,19 +435,25 @@ class AdamW(torch.optim.Optimizer):
         ids = [i for g in state_dict["param_groups"] for i in g["params"]]
         for i, (p, g) in zip(ids, [(p, g) for g in self.param_groups for p in g["params"]]):
             if i in saved and saved[i]:
-                self._load_one(p, g, saved[i])
+                self._load_one(i, p, g, saved[i])
 
-    def _load_one(self, p, group, saved):
+    def _load_one(self, i, p, group, saved):
+        for k in ("step", "exp_avg", "exp_avg_sq"):
+            if k not in saved:
+                raise ValueError(f"state of parameter {i}: {k} is missing")
         step = float(saved["step"])
         s = self._state_of(p, group)
         s["step"].fill_(step)
         put = {k: saved[k].detach().to(p.device) for k in ("exp_avg", "exp_avg_sq", "scales") if k in saved}
         nb = _blocks(p.numel())
         coded = {"exp_avg": (nb, BLOCK), "exp_avg_sq": (nb, BLOCK), "scales": (nb, 2)}
+        types = {"exp_avg": torch.int8, "exp_avg_sq": torch.uint8, "scales": torch.float32}
         for k, x in put.items():
             want = coded[k] if "scales" in put else tuple(p.shape)
             if tuple(x.shape) != want:
-                raise ValueError(f"state {k}: {tuple(x.shape)} for a parameter of {tuple(p.shape)}")
+                raise ValueError(f"state of parameter {i}: {k} of shape {tuple(x.shape)} for a parameter of {tuple(p.shape)}")
+            if x.dtype != types[k] if "scales" in put else not x.is_floating_point():
+                raise ValueError(f"state of parameter {i}: {k} of type {x.dtype}")
         if "scales" in s and "scales" not in put:
             like = torch.empty_like(p, dtype=torch.float32, requires_grad=False)
             m, v = (like.clone().copy_(put[k]) for k in ("exp_avg", "exp_avg_sq"))

@@ -518,3 +518,29 @@ def test_load_state_dict_into_groups_of_their_own(source):
     second.load_state_dict(first.state_dict())
     assert [g["state_bits"] for g in second.param_groups] == [8, 32] and [g["lr"] for g in second.param_groups] == [1e-3, 1e-3]
     assert ["scales" in second.state[p] for p in net.parameters()] == [True] * 3 + [False] * 3
+
+
+@pytest.mark.parametrize("gone", ["step", "exp_avg", "exp_avg_sq"])
+@pytest.mark.parametrize("source", ["torch", 32, 8])
+def test_load_state_dict_refuses_a_state_with_a_part_missing(source, gone):
+    net = networks()
+    first = torch.optim.Adam(net.parameters()) if source == "torch" else optim.AdamW(net.parameters(), state_bits=source, min_8bit_numel=1)
+    train_steps(net, first, 1)
+    saved = first.state_dict()
+    saved["state"][2] = {k: v for k, v in saved["state"][2].items() if k != gone}
+    for bits in (32, 8):
+        with pytest.raises(ValueError, match=f"parameter 2.*{gone}"):
+            optim.AdamW(networks().parameters(), state_bits=bits, min_8bit_numel=1).load_state_dict(saved)
+
+
+def test_load_state_dict_refuses_codes_of_another_type():
+    """Codes that a cast made numbers of another type are no codes."""
+    net = networks()
+    first = optim.AdamW(net.parameters(), state_bits=8, min_8bit_numel=1)
+    train_steps(net, first, 1)
+    for k, t in (("exp_avg", torch.float32), ("exp_avg_sq", torch.int8), ("scales", torch.bfloat16)):
+        saved = first.state_dict()
+        saved["state"][2] = {**saved["state"][2], k: saved["state"][2][k].to(t)}
+        for bits in (32, 8):
+            with pytest.raises(ValueError, match="parameter 2"):
+                optim.AdamW(networks().parameters(), state_bits=bits, min_8bit_numel=1).load_state_dict(saved)
