@@ -393,21 +393,25 @@ class AdamW(torch.optim.Optimizer):
     def _in_8_bits(p, group):
         return group["state_bits"] == 8 and p.numel() >= group["min_8bit_numel"]
 
+    def _new_state(self, p, group):
+        if p.is_cuda and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("a parameter's first step cannot be captured: every replay would clear its moments; take "
+                               "one step before the capture")
+        s = {"step": torch.zeros((), dtype=torch.float32, device=p.device)}
+        if self._in_8_bits(p, group):
+            nb = _blocks(p.numel())
+            s["exp_avg"] = torch.zeros(nb, BLOCK, dtype=torch.int8, device=p.device)
+            s["exp_avg_sq"] = torch.zeros(nb, BLOCK, dtype=torch.uint8, device=p.device)
+            s["scales"] = torch.zeros(nb, 2, dtype=torch.float32, device=p.device)
+        else:
+            for k in ("exp_avg", "exp_avg_sq"):
+                s[k] = torch.zeros_like(p, dtype=torch.float32, requires_grad=False, memory_format=torch.preserve_format)
+        return s
+
     def _state_of(self, p, group):
         s = self.state[p]
         if not s:
-            if p.is_cuda and torch.cuda.is_current_stream_capturing():
-                raise RuntimeError("a parameter's first step cannot be captured: every replay would clear its moments; take "
-                                   "one step before the capture")
-            s["step"] = torch.zeros((), dtype=torch.float32, device=p.device)
-            if self._in_8_bits(p, group):
-                nb = _blocks(p.numel())
-                s["exp_avg"] = torch.zeros(nb, BLOCK, dtype=torch.int8, device=p.device)
-                s["exp_avg_sq"] = torch.zeros(nb, BLOCK, dtype=torch.uint8, device=p.device)
-                s["scales"] = torch.zeros(nb, 2, dtype=torch.float32, device=p.device)
-            else:
-                for k in ("exp_avg", "exp_avg_sq"):
-                    s[k] = torch.zeros_like(p, dtype=torch.float32, requires_grad=False, memory_format=torch.preserve_format)
+            s.update(self._new_state(p, group))
         return s
 
     @torch.no_grad()
@@ -421,29 +425,41 @@ class AdamW(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict):
         """Takes what state_dict() of this class, torch.optim.Adam or torch.optim.AdamW returns; state_bits and min_8bit_numel
-        of the groups stay this optimizer's, and the moments are converted to them."""
-        for g in state_dict["param_groups"]:
-            if g.get("amsgrad") or g.get("maximize"):
-                raise ValueError("amsgrad and maximize are not supported")
-            if g.get("weight_decay") and not g.get("decoupled_weight_decay", True):
-                raise ValueError("the weight decay of torch.optim.Adam (added to the gradient) is not supported")
-        saved = state_dict["state"]
+        of the groups stay this optimizer's, and the moments are converted to them.  What cannot be taken is refused before
+        anything changes."""
         own = [{k: g[k] for k in ("state_bits", "min_8bit_numel")} for g in self.param_groups]
-        super().load_state_dict({**state_dict, "state": {}})
-        for g, bits in zip(self.param_groups, own):
-            g.update(bits)
-        ids = [i for g in state_dict["param_groups"] for i in g["params"]]
-        for i, (p, g) in zip(ids, [(p, g) for g in self.param_groups for p in g["params"]]):
-            if i in saved and saved[i]:
-                self._load_one(i, p, g, saved[i])
+        states = {}
 
-    def _load_one(self, i, p, group, saved):
+        def convert(_, d):       # the last before the load: sees what other hooks put in place
+            for g in d["param_groups"]:
+                if g.get("amsgrad") or g.get("maximize"):
+                    raise ValueError("amsgrad and maximize are not supported")
+                if g.get("weight_decay") and not g.get("decoupled_weight_decay", True):
+                    raise ValueError("the weight decay of torch.optim.Adam (added to the gradient) is not supported")
+            if [len(g["params"]) for g in d["param_groups"]] == [len(g["params"]) for g in self.param_groups]:
+                ids = (i for g in d["param_groups"] for i in g["params"])
+                for i, (p, g) in zip(ids, [(p, g) for g in self.param_groups for p in g["params"]]):
+                    if d["state"].get(i):
+                        states[p] = self._converted(i, p, g, d["state"][i])
+            return {**d, "state": {}}            # the load itself would cast codes to the parameters' type
+
+        def put(_):              # the first after it
+            for g, bits in zip(self.param_groups, own):
+                g.update(bits)
+            self.state.update(states)
+        hooks = (self.register_load_state_dict_pre_hook(convert), self.register_load_state_dict_post_hook(put, prepend=True))
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            for hook in hooks:
+                hook.remove()
+
+    @torch.no_grad()
+    def _converted(self, i, p, group, saved):
+        """A state of p, in its group's number of bits, of the saved one."""
         for k in ("step", "exp_avg", "exp_avg_sq"):
             if k not in saved:
                 raise ValueError(f"state of parameter {i}: {k} is missing")
-        step = float(saved["step"])
-        s = self._state_of(p, group)
-        s["step"].fill_(step)
         put = {k: saved[k].detach().to(p.device) for k in ("exp_avg", "exp_avg_sq", "scales") if k in saved}
         nb = _blocks(p.numel())
         coded = {"exp_avg": (nb, BLOCK), "exp_avg_sq": (nb, BLOCK), "scales": (nb, 2)}
@@ -454,6 +470,8 @@ class AdamW(torch.optim.Optimizer):
                 raise ValueError(f"state of parameter {i}: {k} of shape {tuple(x.shape)} for a parameter of {tuple(p.shape)}")
             if x.dtype != types[k] if "scales" in put else not x.is_floating_point():
                 raise ValueError(f"state of parameter {i}: {k} of type {x.dtype}")
+        s = self._new_state(p, group)
+        s["step"].fill_(float(saved["step"]))
         if "scales" in s and "scales" not in put:
             like = torch.empty_like(p, dtype=torch.float32, requires_grad=False)
             m, v = (like.clone().copy_(put[k]) for k in ("exp_avg", "exp_avg_sq"))
@@ -463,6 +481,7 @@ class AdamW(torch.optim.Optimizer):
             put = {k: x.reshape(-1)[:p.numel()].as_strided(p.shape, p.stride()) for k, x in (("exp_avg", m), ("exp_avg_sq", v))}
         for k, x in put.items():
             s[k].copy_(x)
+        return s
 
 
 @torch.no_grad()

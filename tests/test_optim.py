@@ -544,3 +544,47 @@ def test_load_state_dict_refuses_codes_of_another_type():
         for bits in (32, 8):
             with pytest.raises(ValueError, match="parameter 2"):
                 optim.AdamW(networks().parameters(), state_bits=bits, min_8bit_numel=1).load_state_dict(saved)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_load_state_dict_that_fails_changes_nothing(bits):
+    net, other = networks(), networks(3)
+    first = optim.AdamW(net.parameters(), lr=5e-3)
+    train_steps(net, first, 2)
+    second = optim.AdamW(other.parameters(), lr=1e-3, state_bits=bits, min_8bit_numel=100)
+    train_steps(other, second, 1)
+    before = [(p, k, x, x.clone() if torch.is_tensor(x) else x) for p, s in second.state.items() for k, x in s.items()]
+    for change in (lambda d: d["state"].update({5: {**d["state"][5], "exp_avg_sq": torch.zeros(2)}}),
+                   lambda d: d["state"].update({5: {"step": torch.tensor(1.0)}}),
+                   lambda d: d["param_groups"][0].update(amsgrad=True),
+                   lambda d: d["param_groups"][0]["params"].pop()):
+        saved = first.state_dict()
+        change(saved)
+        with pytest.raises(ValueError):
+            second.load_state_dict(saved)
+        assert second.param_groups[0]["lr"] == 1e-3 and len(second.state) == 6
+        for p, k, x, y in before:
+            now = second.state[p][k]
+            assert now is x and (torch.equal(x, y) if torch.is_tensor(x) else x == y)
+
+
+def test_load_state_dict_hooks_see_the_states():
+    """Hooks before the load may put another state in place; hooks after it find the loaded one."""
+    net = networks()
+    first = optim.AdamW(net.parameters(), lr=1e-3)
+    train_steps(net, first, 2)
+    second = optim.AdamW(networks().parameters(), state_bits=8, min_8bit_numel=100)
+    seen = []
+
+    def before(opt, d):
+        return {**d, "state": {k: {**s, "step": s["step"] + 40} for k, s in d["state"].items()}}
+
+    def after(opt):
+        seen.append([(float(opt.state[p]["step"]), "scales" in opt.state[p], opt.param_groups[0]["state_bits"])
+                     for p in opt.param_groups[0]["params"]])
+    second.register_load_state_dict_pre_hook(before)
+    second.register_load_state_dict_post_hook(after)
+    second.load_state_dict(first.state_dict())
+    assert seen == [[(42.0, p.numel() >= 100, 8) for p in net.parameters()]]
+    second.load_state_dict(first.state_dict())           # nothing of the load stays behind
+    assert len(seen) == 2 and len(second._optimizer_load_state_dict_pre_hooks) == len(second._optimizer_load_state_dict_post_hooks) == 1
