@@ -66,6 +66,20 @@ bool coded(const at::Tensor& q, const at::Tensor& c, const at::Tensor& s, long n
          !((size_t)address(s) & 7);
 }
 
+// whether p's elements lie in the order that the state of its codes records, if it does
+bool same_order(const at::Tensor& p, PyObject* state) {
+  static PyObject* const key = PyUnicode_InternFromString("strides");
+  PyObject* strides = PyDict_Check(state) ? PyDict_GetItem(state, key) : nullptr;
+  if (!strides) return true;
+  if (!PyTuple_Check(strides) || PyTuple_GET_SIZE(strides) != p.dim()) return false;
+  for (int64_t k = 0; k < p.dim(); ++k) {
+    const long x = PyLong_AsLong(PyTuple_GET_ITEM(strides, k));
+    if (x == -1 && PyErr_Occurred()) PyErr_Clear();
+    if (p.size(k) != 1 && p.stride(k) != x) return false;
+  }
+  return true;
+}
+
 // The memory of a step's tensors, in lists that are written (parameters, both moments, scales, step counts) or only read
 // (gradients).  No byte that is written may belong to two tensors; those that are only read may share theirs.
 class Memory {
@@ -158,20 +172,21 @@ PyObject* fail(const char* what, int code) {
 
 // adamw_step(fn, bytes_fn, params, grads, exp_avgs, exp_avg_sqs, scales | None, steps: tensor or list, groups: address of
 // an int for each tensor | 0, list of (lr, beta1, beta2, eps, weight decay, address of the lr on the device | 0),
-// max_norm, skip_nonfinite, want_norm, device index, stream) -> norm | None
+// max_norm, skip_nonfinite, want_norm, device index, stream, states: list of dictionaries | None) -> norm | None
 PyObject* step(PyObject*, PyObject* args) {
   unsigned long long fn, bytes_fn, groups_at, stream;
-  PyObject *params, *grads, *ms, *vs, *ss, *ts, *hypers;
+  PyObject *params, *grads, *ms, *vs, *ss, *ts, *hypers, *states;
   int skip, want, index;
   double max_norm;
-  if (!PyArg_ParseTuple(args, "KKOOOOOOKO!dppiK", &fn, &bytes_fn, &params, &grads, &ms, &vs, &ss, &ts, &groups_at,
-                        &PyList_Type, &hypers, &max_norm, &skip, &want, &index, &stream))
+  if (!PyArg_ParseTuple(args, "KKOOOOOOKO!dppiKO", &fn, &bytes_fn, &params, &grads, &ms, &vs, &ss, &ts, &groups_at,
+                        &PyList_Type, &hypers, &max_norm, &skip, &want, &index, &stream, &states))
     return nullptr;
   try {
     const c10::Device dev(c10::kCUDA, (c10::DeviceIndex)index);
-    const Items P(params), G(grads), M(ms), V(vs), S(ss), T(ts);
+    const Items P(params), G(grads), M(ms), V(vs), S(ss), T(ts), D(states);
     const Py_ssize_t n = P.n;
-    if (n < 1 || G.n != n || M.n != n || V.n != n || (ss != Py_None && S.n != n)) Py_RETURN_NOTIMPLEMENTED;
+    if (n < 1 || G.n != n || M.n != n || V.n != n || (ss != Py_None && S.n != n) || (D.n >= 0 && D.n != n))
+      Py_RETURN_NOTIMPLEMENTED;
     Lists a;
     for (auto* x : {&a.p, &a.g, &a.m, &a.v, &a.s, &a.t}) x->resize(n);
     a.numels.resize(n);
@@ -195,7 +210,7 @@ PyObject* step(PyObject*, PyObject* args) {
       } else {
         const at::Tensor* s = tensor_of(so, dev);
         const long nb = (numel + 255) / 256;
-        if (!s || !coded(*m, *v, *s, nb)) Py_RETURN_NOTIMPLEMENTED;
+        if (!s || !coded(*m, *v, *s, nb) || (D.n >= 0 && !same_order(*p, D.at[i]))) Py_RETURN_NOTIMPLEMENTED;
         as = address(*s);
         if (!as) as = (char*)16;                 // no blocks: 8-bit all the same
         memory.add(Memory::kFirst, am, 256 * nb);

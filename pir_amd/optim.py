@@ -71,16 +71,29 @@ def _max_norm(max_norm):
     return max_norm if max_norm < math.inf else 0.0
 
 
-def _dense(t):
-    """Whether t's elements fill one stretch of memory, each once, in some order of its dimensions."""
-    if t.is_contiguous():
-        return True
+def _fills(shape, strides):
+    """Whether elements with these strides fill one stretch of memory, each once, in some order of the dimensions."""
     want = 1
-    for size, stride in sorted(((s, d) for s, d in zip(t.shape, t.stride()) if s != 1), key=lambda x: x[1]):
+    for size, stride in sorted(((s, d) for s, d in zip(shape, strides) if s != 1), key=lambda x: x[1]):
         if stride != want:
             return False
         want *= size
     return True
+
+
+def _dense(t):
+    return t.is_contiguous() or _fills(t.shape, t.stride())
+
+
+def _same_order(shape, a, b):
+    return all(x == y for n, x, y in zip(shape, a, b) if n != 1)
+
+
+def _check_orders(params, states):
+    """Codes follow their parameter's order of memory as it was when they came to be ("strides", where it is recorded)."""
+    for p, s in zip(params, states):
+        if "scales" in s and "strides" in s and not _same_order(p.shape, p.stride(), s["strides"]):
+            raise ValueError(f"the order of a parameter's memory changed: strides {p.stride()}, of its 8-bit moments {s['strides']}")
 
 
 def _blocks(numel):
@@ -171,15 +184,16 @@ def _stream(dev):
     return torch._C._cuda_getCurrentRawStream(dev.index)
 
 
-def _run(params, grads, exp_avgs, exp_avg_sqs, scales, steps, groups, hypers, max_norm, skip_nonfinite, want_norm):
+def _run(params, grads, exp_avgs, exp_avg_sqs, scales, steps, groups, hypers, max_norm, skip_nonfinite, want_norm, states=None):
     """One pir_adamw_step.  steps: a tensor with one count per parameter, or a list of them; groups: index into hypers of
-    each tensor, an array of int (None: all in the first)."""
+    each tensor, an array of int (None: all in the first); states: the optimizer's, whose codes record their order."""
     dev = params[0].device
     host, step, size, *_ = _host()
     rest = (exp_avgs, exp_avg_sqs, scales, steps, 0 if groups is None else groups.buffer_info()[0], hypers, max_norm,
-            skip_nonfinite, want_norm, dev.index, _stream(dev))
+            skip_nonfinite, want_norm, dev.index, _stream(dev), states)
     norm = host.adamw_step(step, size, params, grads, *rest)
     if norm is NotImplemented:
+        _check_orders(params, states or ())
         grads = _check(params, grads, exp_avgs, exp_avg_sqs, scales, steps)
         norm = host.adamw_step(step, size, params, grads, *rest)
         if norm is NotImplemented:
@@ -359,8 +373,9 @@ class AdamW(torch.optim.Optimizer):
     they are in a step whose joint norm is not finite.  Either leaves the norm before clipping in total_norm, a
     device tensor.  A parameter without a gradient is skipped: no state, no step counted.
 
-    state[p]: "step" (fp32, on p's device), "exp_avg", "exp_avg_sq" and, in 8 bits, "scales".  load_state_dict takes the
-    states of torch.optim.Adam and AdamW too, and converts between 32 and 8 bits as this optimizer's groups ask for."""
+    state[p]: "step" (fp32, on p's device), "exp_avg", "exp_avg_sq" and, in 8 bits, "scales" and the "strides" of p, whose
+    order of memory the codes follow.  load_state_dict takes the states of torch.optim.Adam and AdamW too, and converts
+    between 32 and 8 bits as this optimizer's groups ask for, and between orders of memory."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, min_8bit_numel=4096,
                  max_norm=None, skip_nonfinite=False):
@@ -403,6 +418,7 @@ class AdamW(torch.optim.Optimizer):
             s["exp_avg"] = torch.zeros(nb, BLOCK, dtype=torch.int8, device=p.device)
             s["exp_avg_sq"] = torch.zeros(nb, BLOCK, dtype=torch.uint8, device=p.device)
             s["scales"] = torch.zeros(nb, 2, dtype=torch.float32, device=p.device)
+            s["strides"] = p.stride()
         else:
             for k in ("exp_avg", "exp_avg_sq"):
                 s[k] = torch.zeros_like(p, dtype=torch.float32, requires_grad=False, memory_format=torch.preserve_format)
@@ -470,15 +486,22 @@ class AdamW(torch.optim.Optimizer):
                 raise ValueError(f"state of parameter {i}: {k} of shape {tuple(x.shape)} for a parameter of {tuple(p.shape)}")
             if x.dtype != types[k] if "scales" in put else not x.is_floating_point():
                 raise ValueError(f"state of parameter {i}: {k} of type {x.dtype}")
+        order = saved.get("strides", p.stride())
+        if "scales" in put:
+            if "strides" not in saved and not p.is_contiguous():
+                raise ValueError(f"state of parameter {i}: the order of its codes is not recorded, and the parameter not contiguous")
+            if not isinstance(order, (tuple, list)) or len(order) != p.dim() or not all(isinstance(x, int) for x in order) \
+                    or (p.numel() and not _fills(p.shape, order)):
+                raise ValueError(f"state of parameter {i}: strides {order} are no order of a parameter of {tuple(p.shape)}")
         s = self._new_state(p, group)
         s["step"].fill_(float(saved["step"]))
+        if "scales" in put and not ("scales" in s and _same_order(p.shape, order, p.stride())):
+            m, v = moments8_decode(*(put[k].contiguous() for k in ("exp_avg", "exp_avg_sq", "scales")))
+            put = {k: x.reshape(-1)[:p.numel()].as_strided(p.shape, order) for k, x in (("exp_avg", m), ("exp_avg_sq", v))}
         if "scales" in s and "scales" not in put:
             like = torch.empty_like(p, dtype=torch.float32, requires_grad=False)
             m, v = (like.clone().copy_(put[k]) for k in ("exp_avg", "exp_avg_sq"))
             put = dict(zip(("exp_avg", "exp_avg_sq", "scales"), moments8_encode(m, v)))
-        elif "scales" not in s and "scales" in put:
-            m, v = moments8_decode(*(put[k].contiguous() for k in ("exp_avg", "exp_avg_sq", "scales")))
-            put = {k: x.reshape(-1)[:p.numel()].as_strided(p.shape, p.stride()) for k, x in (("exp_avg", m), ("exp_avg_sq", v))}
         for k, x in put.items():
             s[k].copy_(x)
         return s
@@ -535,5 +558,6 @@ class _Job:
         scales = [s.get("scales") for s in self.states]
         rest = (t, self.groups, self.hypers, bound, skip_nonfinite, want_norm)
         if self.device.type == "cuda":
-            return _run(self.params, grads, m, v, scales, *rest)
+            return _run(self.params, grads, m, v, scales, *rest, self.states)
+        _check_orders(self.params, self.states)
         return _run_torch(self.params, _check(self.params, grads, m, v, scales, t), m, v, scales, *rest)

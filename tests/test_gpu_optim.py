@@ -8,7 +8,7 @@ import torch
 
 import optim_util as U
 from pir_amd import optim, train
-from test_optim import assert_moved_alike, networks, overlaps, refused_call, run, train_steps
+from test_optim import LAYOUTS, assert_moved_alike, check_load_of_another_order, networks, optimizer_of, overlaps, refused_call, run, train_steps
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -638,3 +638,25 @@ def test_small_second_moments_beside_large_ones_keep_a_code(device):
     want = torch.ones(4, 256, dtype=torch.uint8)
     want[:, 0], want[:, 5] = 255, 0
     assert torch.equal(c.cpu(), want)
+
+
+@pytest.mark.parametrize("bits", [(8, 8), (8, 32), (32, 8)])
+@pytest.mark.parametrize("target", LAYOUTS)
+@pytest.mark.parametrize("source", LAYOUTS)
+def test_load_state_dict_into_another_order_of_memory(source, target, bits):
+    check_load_of_another_order(source, target, bits, DEV)
+
+
+def test_a_parameter_whose_order_changes_under_its_codes():
+    opt, p = optimizer_of("contiguous", 8, DEV)
+    p.data = p.data.contiguous(memory_format=torch.channels_last)
+    p.grad = torch.ones_like(p)
+    before = p.detach().clone()
+    with pytest.raises(ValueError, match="order"):
+        opt.step()
+    assert torch.equal(p, before) and float(opt.state[p]["step"]) == 2
+    opt, p = optimizer_of("contiguous", 8, DEV, shape=(8, 16, 1, 1))
+    p.data = p.data.contiguous().as_strided(p.shape, (16, 1, 16, 16))
+    p.grad = torch.ones_like(p)
+    opt.step()
+    assert float(opt.state[p]["step"]) == 3

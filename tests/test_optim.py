@@ -588,3 +588,71 @@ def test_load_state_dict_hooks_see_the_states():
     assert seen == [[(42.0, p.numel() >= 100, 8) for p in net.parameters()]]
     second.load_state_dict(first.state_dict())           # nothing of the load stays behind
     assert len(seen) == 2 and len(second._optimizer_load_state_dict_pre_hooks) == len(second._optimizer_load_state_dict_post_hooks) == 1
+
+
+LAYOUTS = {
+    "contiguous": lambda x: x.contiguous(),
+    "channels_last": lambda x: x.contiguous(memory_format=torch.channels_last),
+    "transposed": lambda x: x.permute(3, 2, 1, 0).contiguous().permute(3, 2, 1, 0),
+}
+
+
+def optimizer_of(layout, bits, device="cpu", steps=2, shape=(8, 16, 6, 6)):
+    """An optimizer of one parameter whose memory is in some order, after some steps."""
+    gen = torch.Generator().manual_seed(1)
+    p = torch.nn.Parameter(LAYOUTS[layout](torch.randn(shape, generator=gen)).to(device))
+    opt = optim.AdamW([p], lr=1e-3, state_bits=bits, min_8bit_numel=1)
+    for _ in range(steps):
+        p.grad = LAYOUTS[layout](torch.randn(shape, generator=gen) * torch.exp(torch.randn(shape, generator=gen))).to(device)
+        opt.step()
+    return opt, p
+
+
+def check_load_of_another_order(source, target, bits, device):
+    a, pa = optimizer_of(source, bits[0], device)
+    b, pb = optimizer_of(target, bits[1], device, steps=0)
+    assert pa.stride() == LAYOUTS[source](pa).stride() and pb.stride() == LAYOUTS[target](pb).stride()
+    b.load_state_dict(a.state_dict())
+    # in another order other elements share a scale, so codes are rounded once more: to the nearest of the new block's
+    parts = CODE_PARTS if bits[1] == 8 and (bits[0] == 32 or source != target) else (1e-6, 1e-6) if bits[0] != bits[1] else (0.0, 0.0)
+    assert_same_moments(a, pa, b, pb, parts)
+
+
+@pytest.mark.parametrize("bits", [(8, 8), (8, 32), (32, 8), (32, 32)])
+@pytest.mark.parametrize("target", LAYOUTS)
+@pytest.mark.parametrize("source", LAYOUTS)
+def test_load_state_dict_into_another_order_of_memory(source, target, bits):
+    check_load_of_another_order(source, target, bits, "cpu")
+
+
+def test_codes_without_a_record_of_their_order():
+    """They are of a contiguous parameter: another cannot take them."""
+    a, _ = optimizer_of("contiguous", 8)
+    saved = a.state_dict()
+    del saved["state"][0]["strides"]
+    b, _ = optimizer_of("contiguous", 8, steps=0)
+    b.load_state_dict(saved)
+    for bits in (8, 32):
+        c, _ = optimizer_of("channels_last", bits, steps=0)
+        with pytest.raises(ValueError, match="order"):
+            c.load_state_dict(saved)
+    for bad in ((1, 1, 1, 1), (576, 36, 6, 2), (576, 36, 6), None, (-576, 36, 6, 1)):
+        with pytest.raises(ValueError, match="order"):
+            b.load_state_dict({**saved, "state": {0: {**saved["state"][0], "strides": bad}}})
+
+
+def test_a_parameter_whose_order_changes_under_its_codes():
+    """module.to(memory_format=...) moves a parameter's elements; codes cannot follow, and the step says so."""
+    opt, p = optimizer_of("contiguous", 8)
+    p.data = p.data.contiguous(memory_format=torch.channels_last)
+    p.grad = torch.ones_like(p)
+    before = p.detach().clone()
+    with pytest.raises(ValueError, match="order"):
+        opt.step()
+    assert torch.equal(p, before)
+    # strides of dimensions of one element say nothing
+    opt, p = optimizer_of("contiguous", 8, shape=(8, 16, 1, 1))
+    p.data = p.data.contiguous().as_strided(p.shape, (16, 1, 16, 16))
+    p.grad = torch.ones_like(p)
+    opt.step()
+    assert float(opt.state[p]["step"]) == 3
