@@ -270,7 +270,8 @@ typedef struct PirAdamwGroup {
   const float* lr_device;
 } PirAdamwGroup;
 
-/* Workspace of pir_adamw_step; with_norm: max_norm > 0, skip_nonfinite or total_norm is asked for. */
+/* Bytes of pir_adamw_step's workspace, which has to start at a multiple of 16; with_norm: max_norm > 0, skip_nonfinite
+ * or total_norm is asked for. */
 size_t pir_adamw_workspace_bytes(int n, const long* numels, int with_norm);
 
 /* One step of n tensors.  Every array is a HOST array of n entries; params, grads, exp_avgs, exp_avg_sqs, scales and
@@ -281,17 +282,19 @@ size_t pir_adamw_workspace_bytes(int n, const long* numels, int with_norm);
  * params[i] and grads[i]: numels[i] values of type dtypes[i].  scales NULL or scales[i] NULL: exp_avgs[i] and
  * exp_avg_sqs[i] are fp32[numels[i]].  Otherwise they are 8-bit codes, int8 and uint8 [ceil(numels[i] / 256) * 256],
  * and scales[i] is fp32 [ceil(numels[i] / 256)][2]: m = s0 (q / 127) |q / 127|, v = s1 (c / 255)^4, s0 and s1 the
- * largest |m| and v of 256 consecutive elements (codes aligned to 16 bytes, scales to 8; what lies behind numels[i] is written as zero).  A
- * moment that is not finite makes its block's scale NaN, a second one both scales; eps has to be 1e-30 at least.  groups[i]: index into group.  skip_nonfinite: if |g| is not
- * finite nothing changes, the step counts included.  total_norm: optional DEVICE float that receives |g|.
- * No two tensors of a call may overlap, step counts included. */
+ * largest |m| and v of 256 consecutive elements (codes aligned to 16 bytes, scales to 8; what lies behind numels[i] is
+ * written as zero).  A moment that is not finite makes its block's scale NaN, a second one both scales; eps has to be
+ * 1e-30 at least.  groups[i]: index into group.  skip_nonfinite: if |g| is not finite nothing changes, the step counts
+ * included.  total_norm: optional DEVICE float that receives |g|.
+ * Nothing that is written may overlap another tensor of the call, step counts included: the caller sees to it. */
 int pir_adamw_step(int n, void* const* params, const void* const* grads, void* const* exp_avgs, void* const* exp_avg_sqs,
                    float* const* scales, float* const* steps, const long* numels, const int* dtypes, const int* groups,
                    const PirAdamwGroup* group, int n_groups, double max_norm, int skip_nonfinite, float* total_norm,
                    void* workspace, size_t workspace_bytes, void* stream);
 
 /* 2-norms of n tensors: *total (DEVICE) of all of them together, each[n] (DEVICE, or NULL) of every one.  Squares and
- * sums in 64 bits, in a fixed order.  grads, numels, dtypes: HOST arrays as above. */
+ * sums in 64 bits, in a fixed order.  grads, numels, dtypes: HOST arrays as above.  The workspace has to start at a multiple
+ * of 8. */
 size_t pir_grad_norm_workspace_bytes(int n, const long* numels);
 int pir_grad_norm(int n, const void* const* grads, const long* numels, const int* dtypes, float* total, float* each,
                   void* workspace, size_t workspace_bytes, void* stream);

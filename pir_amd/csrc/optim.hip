@@ -721,7 +721,8 @@ int pir_adamw_step(int n, void* const* params, const void* const* grads, void* c
   if (n > 0 && (!params || !exp_avgs || !exp_avg_sqs || !steps || !groups || !group || n_groups < 1)) return PIR_ERR_ARG;
   for (int k = 0; k < n_groups && n > 0; ++k) {
     const PirAdamwGroup& g = group[k];
-    if (!(g.beta1 >= 0 && g.beta1 < 1 && g.beta2 >= 0 && g.beta2 < 1 && g.eps >= 0 && g.lr >= 0 && g.weight_decay >= 0))
+    if (!(g.beta1 >= 0 && g.beta1 < 1 && g.beta2 >= 0 && g.beta2 < 1 && g.eps >= 0 && g.lr >= 0 && g.weight_decay >= 0) ||
+        ((size_t)g.lr_device & 3))
       return PIR_ERR_ARG;
   }
   for (int i = 0; i < n; ++i) {
@@ -734,9 +735,10 @@ int pir_adamw_step(int n, void* const* params, const void* const* grads, void* c
       return PIR_ERR_ARG;
   }
   const bool clip = max_norm > 0.0, with_norm = clip || skip_nonfinite || total_norm;
+  if ((size_t)total_norm & 3) return PIR_ERR_ARG;
   if (n == 0 && !total_norm) return PIR_OK;
   const StepSpace space(n, numels, with_norm);
-  if (!workspace || workspace_bytes < (size_t)space.bytes) return PIR_ERR_SCRATCH;
+  if (!workspace || ((size_t)workspace & 15) || workspace_bytes < (size_t)space.bytes) return PIR_ERR_SCRATCH;
   char* ws = (char*)workspace;
   OptRow* rows = (OptRow*)(ws + space.rows);
   OptCoef* coef = (OptCoef*)(ws + space.coef);
@@ -819,8 +821,8 @@ int pir_grad_norm(int n, const void* const* grads, const long* numels, const int
   hipStream_t stream = (hipStream_t)stream_;
   const int rc = check_tensors(n, numels, dtypes, grads, nullptr);
   if (rc != PIR_OK) return rc;
-  if (!total) return PIR_ERR_ARG;
-  if (!workspace || workspace_bytes < pir_grad_norm_workspace_bytes(n, numels)) return PIR_ERR_SCRATCH;
+  if (!total || (((size_t)total | (size_t)each) & 3)) return PIR_ERR_ARG;
+  if (!workspace || ((size_t)workspace & 7) || workspace_bytes < pir_grad_norm_workspace_bytes(n, numels)) return PIR_ERR_SCRATCH;
   const long n_partial = norm_partials(n, numels);
   double* partial = (double*)workspace;
   if (launch_partials(n, grads, numels, dtypes, partial, stream) != PIR_OK) return PIR_ERR_LAUNCH;
@@ -851,7 +853,8 @@ int pir_moments8_decode(long n_blocks, const signed char* exp_avg, const unsigne
   if (n_blocks < 0 || dtype < PIR_F32 || dtype > PIR_F16) return PIR_ERR_ARG;
   if (n_blocks > kMaxGroups * (kOptChunk8 / kOptBlock)) return PIR_ERR_TOO_LARGE;
   if (n_blocks == 0) return PIR_OK;
-  if (!exp_avg || !exp_avg_sq || !scales || !m || !v || ((((size_t)exp_avg | (size_t)exp_avg_sq) & 15) || ((size_t)scales & 7)))
+  if (!exp_avg || !exp_avg_sq || !scales || !m || !v || ((((size_t)exp_avg | (size_t)exp_avg_sq) & 15) || ((size_t)scales & 7)) ||
+      (((size_t)m | (size_t)v) & (element_bytes(dtype) - 1)))
     return PIR_ERR_ARG;
   const dim3 grid((unsigned)ceil_div(n_blocks * kOptBlock, kOptChunk8)), block(kOptThreads);
   hipStream_t s = (hipStream_t)stream;
@@ -869,7 +872,8 @@ int pir_moments8_encode(long numel, int dtype, const void* m, const void* v, sig
   if (numel < 0 || dtype < PIR_F32 || dtype > PIR_F16) return PIR_ERR_ARG;
   if (numel > kMaxGroups * kOptChunk8) return PIR_ERR_TOO_LARGE;
   if (numel == 0) return PIR_OK;
-  if (!exp_avg || !exp_avg_sq || !scales || !m || !v || ((((size_t)exp_avg | (size_t)exp_avg_sq) & 15) || ((size_t)scales & 7)))
+  if (!exp_avg || !exp_avg_sq || !scales || !m || !v || ((((size_t)exp_avg | (size_t)exp_avg_sq) & 15) || ((size_t)scales & 7)) ||
+      (((size_t)m | (size_t)v) & (element_bytes(dtype) - 1)))
     return PIR_ERR_ARG;
   const dim3 grid((unsigned)ceil_div(numel, kOptChunk8)), block(kOptThreads);
   hipStream_t s = (hipStream_t)stream;

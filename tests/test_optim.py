@@ -656,3 +656,24 @@ def test_a_parameter_whose_order_changes_under_its_codes():
     p.grad = torch.ones_like(p)
     opt.step()
     assert float(opt.state[p]["step"]) == 3
+
+
+@pytest.mark.parametrize("code, change", [
+    (3, dict(work=4104, size=1 << 20)), (3, dict(work=4097, size=1 << 20)),     # descriptors are read from it 16 bytes at a time
+    (1, dict(norm=4098, size=1 << 20)), (1, dict(group=(Group * 1)(Group(1e-3, 0.9, 0.99, 1e-8, 0.0, 4097)), size=1 << 20)),
+])
+def test_c_step_refuses_what_is_not_aligned(code, change):
+    assert c_step(**change) == code
+
+
+def test_c_calls_refuse_what_is_not_aligned():
+    from pir_amd import _lib
+    L = _lib.lib()
+    one, numels, f32 = (ctypes.c_void_p * 1)(4096), (ctypes.c_long * 1)(10), (ctypes.c_int * 1)(0)
+    at = [ctypes.addressof(x) for x in (one, numels, f32)]
+    for total, each, work, code in ((4098, None, 4096, 1), (4096, 4097, 4096, 1), (4096, None, 4100, 3)):
+        assert L.pir_grad_norm(1, *at, total, each, work, 1 << 16, None) == code
+    for dtype, bad in ((0, 4098), (1, 4097), (2, 4097)):
+        for m, v in ((bad, 4096), (4096, bad)):
+            assert L.pir_moments8_decode(1, 4096, 4096, 4096, dtype, m, v, None) == 1
+            assert L.pir_moments8_encode(5, dtype, m, v, 4096, 4096, 4096, None) == 1
