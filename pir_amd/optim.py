@@ -336,6 +336,7 @@ def moments8_encode(exp_avg, exp_avg_sq):
         numel, nb, dev = m.numel(), _blocks(m.numel()), m.device
         if dev.type != "cuda":
             return _encode_torch(m.as_strided((numel,), (1,)), v.as_strided((numel,), (1,)))
+        m, v = m.resolve_neg(), v.resolve_neg()
         out = (torch.empty(nb, BLOCK, dtype=torch.int8, device=dev), torch.empty(nb, BLOCK, dtype=torch.uint8, device=dev),
                torch.empty(nb, 2, dtype=torch.float32, device=dev))
         with torch.cuda.device(dev):

@@ -660,3 +660,21 @@ def test_a_parameter_whose_order_changes_under_its_codes():
     p.grad = torch.ones_like(p)
     opt.step()
     assert float(opt.state[p]["step"]) == 3
+
+
+@pytest.mark.parametrize("device", ["cpu", DEV])
+def test_negated_views_are_taken_by_value(device):
+    """A view that torch keeps as "the negative of this memory" (the imaginary part of a conjugate) is its values."""
+    x = torch.randn(600, generator=torch.Generator().manual_seed(0)).to(device)
+    neg = torch._neg_view(x)
+    assert neg.is_neg() and torch.equal(neg, -x)
+    for got, want in zip(optim.moments8_encode(neg, x.abs()), optim.moments8_encode(-x, x.abs())):
+        assert torch.equal(got, want)
+    for got, want in zip(optim.grad_norm([neg]), optim.grad_norm([x])):
+        assert torch.equal(got, want)
+    ends = []
+    for g in (neg, -x):
+        p = [torch.ones(600, device=device)]
+        optim.adamw_step(p, [g], [torch.zeros(600, device=device)], [torch.zeros(600, device=device)], torch.zeros(1, device=device), lr=1e-2)
+        ends.append(p[0])
+    assert torch.equal(*ends)
