@@ -278,7 +278,7 @@ def adamw8_step(params, grads, exp_avgs, exp_avg_sqs, scales, steps, *, lr, beta
 
 def _check_norm(tensors, dev):
     for i, t in enumerate(tensors):
-        if t.dtype not in _DTYPES or t.layout is not torch.strided or t.device != dev:
+        if not isinstance(t, torch.Tensor) or t.dtype not in _DTYPES or t.layout is not torch.strided or t.device != dev:
             raise ValueError(f"tensor {i}: dense float32, bfloat16 or float16 on the device of tensor 0 is wanted")
 
 
@@ -288,9 +288,9 @@ def grad_norm(tensors):
     tensors = list(tensors)
     if not tensors:
         raise ValueError("grad_norm: no tensors")
-    dev = tensors[0].device
+    dev = getattr(tensors[0], "device", None)
     with torch.no_grad():
-        if dev.type != "cuda":
+        if dev is None or dev.type != "cuda":
             _check_norm(tensors, dev)
             each = torch.stack([t.double().square().sum() for t in tensors])
             return each.sum().sqrt().float(), each.sqrt().float()

@@ -677,3 +677,10 @@ def test_c_calls_refuse_what_is_not_aligned():
         for m, v in ((bad, 4096), (4096, bad)):
             assert L.pir_moments8_decode(1, 4096, 4096, 4096, dtype, m, v, None) == 1
             assert L.pir_moments8_encode(5, dtype, m, v, 4096, 4096, 4096, None) == 1
+
+
+@pytest.mark.parametrize("bad", [[None], [torch.ones(3), None], [torch.ones(3), 2.0]])
+def test_grad_norm_refuses_what_is_no_tensor(bad):
+    """A parameter without a gradient, above all: leaving it out is the caller's."""
+    with pytest.raises(ValueError, match=f"tensor {len(bad) - 1}"):
+        optim.grad_norm(bad)
