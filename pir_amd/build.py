@@ -37,6 +37,7 @@ def build(force=False, verbose=True):
     hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
     headers = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith((".cuh", ".h"))]
     headers.append(os.path.join(HERE, "..", "include", "pir_hip.h"))
+    own = os.path.abspath(__file__)              # its flags: objects of other ones are stale too
     objs = []
     procs = []
     for src in SOURCES:
@@ -45,13 +46,13 @@ def build(force=False, verbose=True):
             continue
         obj = os.path.join(CSRC, src.replace(".hip", ".o"))
         objs.append(obj)
-        if force or _stale(obj, [path] + headers):
+        if force or _stale(obj, [path, own] + headers):
             cmd = [hipcc] + FLAGS + ["-c", path, "-o", obj]
             if verbose:
                 print(" ".join(cmd), flush=True)
             procs.append((src, subprocess.Popen(cmd)))
     compiled = bool(procs)
-    if force or _stale(HOST_OUT, [HOST_SRC, headers[-1]]):
+    if force or _stale(HOST_OUT, [HOST_SRC, own, headers[-1]]):
         cmd = _host_command()
         if verbose:
             print(" ".join(cmd), flush=True)
