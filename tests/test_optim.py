@@ -684,3 +684,20 @@ def test_grad_norm_refuses_what_is_no_tensor(bad):
     """A parameter without a gradient, above all: leaving it out is the caller's."""
     with pytest.raises(ValueError, match=f"tensor {len(bad) - 1}"):
         optim.grad_norm(bad)
+
+
+@pytest.mark.parametrize("bits, what, change", [(bits, *case) for bits, test in ((32, test_step_refuses), (8, test_8_bit_step_refuses))
+                                                for case in test.pytestmark[0].args[1]])
+def test_a_refused_step_leaves_what_it_was_given(bits, what, change):
+    """The very tensors of the call, those put in to have it refused among them: parameters, moments, scales, counts."""
+    args = lists(bits=bits)
+    options = dict(lr=1e-3)
+    for k, f in change.items():
+        x = f(args[k]) if callable(f) else f
+        (args if k in args else options)[k] = args[x] if isinstance(x, str) else x
+    given = [t for v in args.values() for t in (v if isinstance(v, list) else [v]) if isinstance(t, torch.Tensor) and not t.is_sparse]
+    before = [t.clone() for t in given]
+    with pytest.raises(ValueError):
+        (optim.adamw8_step if bits == 8 else optim.adamw_step)(*[args[k] for k in (
+            "params", "grads", "exp_avgs", "exp_avg_sqs", "scales", "steps") if k in args], **options)
+    assert len(given) >= 8 and all(torch.equal(a, b) for a, b in zip(given, before)), what
