@@ -22,6 +22,12 @@ eps is 1e-15 or more, next to which such roots are nothing); one that holds an i
 a step that finds one in v sets both scales so: what a bad gradient does to its own moments in 32 bits, it does to its
 block's in 8.  skip_nonfinite leaves everything as it is in a step whose joint norm is not finite in fp32.
 
+A moment in 8 bits moves against its block's largest only once one step moves it by half a code's step.  So an element
+whose gradients stop while its block goes on keeps 0.5 % of the block's largest m (code 9 with beta1 = 0.9) and its share of
+the largest v (any code, with beta2 = 0.999), where in 32 bits both decay to zero: it goes on moving, a step
+by 5 % of lr if its gradients were a tenth of the largest, by 40 % if a hundredth, by nearly lr if less.  Parameters whose
+elements get gradients now and then (tables, rarely chosen rows) belong in 32 bits.
+
 Step counts live on the device (fp32, one per tensor), so that a step can be captured into a HIP graph and replayed; a
 learning rate that changes between replays is a one-element fp32 device tensor.  Calls enqueue work on the current stream
 of the tensors' device and return without waiting.  Tensors on the CPU take the same formulas in torch operations.

@@ -701,3 +701,26 @@ def test_a_refused_step_leaves_what_it_was_given(bits, what, change):
         (optim.adamw8_step if bits == 8 else optim.adamw_step)(*[args[k] for k in (
             "params", "grads", "exp_avgs", "exp_avg_sqs", "scales", "steps") if k in args], **options)
     assert len(given) >= 8 and all(torch.equal(a, b) for a, b in zip(given, before)), what
+
+
+def test_moments8_of_elements_whose_gradients_stop():
+    """What rounding to the nearest code costs, as the module says it: with beta1 = 0.9 a first moment decays to the code 9
+    (9 sqrt(0.9) = 8.54 rounds back to it), 0.5 % of its block's largest, and stays there; with beta2 = 0.999 no code of a
+    second moment falls by its own decay (255 0.999^(1/4) = 254.94), so v stays what it was of the block's largest."""
+    g = torch.full((512,), 1e-2)
+    g[:8] = 1e-3                                         # these stop; the second block has none that do
+    q, c, s = optim.moments8_encode(torch.zeros(512), torch.zeros(512))
+    p, steps = torch.zeros(512), torch.zeros(1)
+    for t in range(800):
+        if t == 200:
+            g[:8] = 0.0
+            codes = c.clone()
+        optim.adamw8_step([p], [g], [q], [c], [s], steps, lr=1e-3)
+        if t >= 260:
+            assert bool((q[0, :8] == 9).all()) and torch.equal(c, codes)
+    before = p.clone()
+    optim.adamw8_step([p], [g], [q], [c], [s], steps, lr=1e-3)
+    assert 0.03 < float((before - p)[0]) / 1e-3 < 0.06   # 0.005 a over the root of 0.01 b, and a^2 = b: 5 % of lr a step
+    m, v = optim.moments8_decode(q, c, s)
+    assert abs(float(m[0, 0] / m[0, 8]) - (9 / 127) ** 2) < 1e-6 and float(v[0, 0] / v[0, 8]) > 0.009
+    assert torch.equal(p[8:256], p[264:]) and float(p[0]) < 0          # and the others of the block are not touched by it
