@@ -257,10 +257,11 @@ __device__ inline unsigned pack_low_bytes(float a, float b, float c, float d) {
 }
 
 // 8-bit moments: half a wave per block of 256 elements, 8 consecutive ones per lane.  10 bytes an element (16-bit
-// parameters) leave the vector unit about 60 operations each, so the arithmetic is counted: square roots and reciprocals
-// are the hardware's (one ulp), the root of v serves the step and the new code, codes are rounded and packed as bits, and
-// maxima cross lanes without shared memory.  435 M bf16 elements: 0.69 ms, 6.4 TB/s, bound by memory; with IEEE roots and
-// divisions and shuffles through shared memory 1.51 ms.
+// parameters) leave the vector unit about 60 operations each, so the arithmetic is counted (it takes 49): square roots and
+// reciprocals are the hardware's (one ulp; about 5e-6 of the codes differ by one from those of correctly rounded ones), the
+// root of v serves the step and the new code, codes are rounded and packed as bits, and maxima cross lanes without shared
+// memory.  435 M bf16 elements: 0.69 ms, 6.4 TB/s, bound by memory; with IEEE roots and divisions and shuffles through
+// shared memory 1.51 ms.
 template <typename T, bool kStream>
 __global__ void __launch_bounds__(kOptThreads)
 adamw8_kernel(const UpdateArgs args) {
@@ -358,7 +359,7 @@ adamw8_kernel(const UpdateArgs args) {
   if ((threadIdx.x & 31) == 0) *sc = make_float2(na, nb);
 }
 
-// 435 M elements to bf16 (2.6 GB): 0.41 ms, 6.4 TB/s
+// 435 M elements to bf16 (2.6 GB): 0.42 ms, 6.2 TB/s; to fp32 (4.4 GB) 1.64 ms, 2.7 TB/s
 template <typename T>
 __global__ void __launch_bounds__(kOptThreads)
 moments8_decode_kernel(long n_blocks, const signed char* __restrict__ mq, const unsigned char* __restrict__ vq,
@@ -378,6 +379,8 @@ moments8_decode_kernel(long n_blocks, const signed char* __restrict__ mq, const 
   store<true>(v + i, y);
 }
 
+// Guarded loads of one element each, not tuned: a program encodes when it loads or converts a state.  435 M elements of
+// bf16 (2.6 GB): 1.3 ms, 2.0 TB/s; of fp32 (4.4 GB) 1.56 ms, 2.8 TB/s.
 template <typename T>
 __global__ void __launch_bounds__(kOptThreads)
 moments8_encode_kernel(long numel, const T* __restrict__ m, const T* __restrict__ v, signed char* __restrict__ mq,

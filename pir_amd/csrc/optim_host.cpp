@@ -1,6 +1,6 @@
 // Host half of pir_amd.optim: reads lists of tensors into the arrays that pir_adamw_step and pir_grad_norm take, and
 // calls them.  One step of the reference's networks has some hundred tensors in each of four lists; reading their types,
-// strides and addresses through Python takes 3 us a tensor, here 0.1 us.
+// strides and addresses through Python takes 3 us a tensor, here 0.1 us; whether they overlap is found out here too.
 //
 // Every function answers NotImplemented where the tensors are not as the kernels want them.  The Python side then says
 // what is wrong, or brings them into order and calls again.
@@ -124,7 +124,7 @@ class Memory {
   }
 
   // Lists that are in the order of memory and apart from all others (views of a buffer each) need no more than their
-  // ends.  Others, as a model's parameters and their states lie, are merged in that order: 7 us for 500 tensors.
+  // ends.  Others, as a model's parameters and their states lie, are merged in that order: 4 us for the 500 of a training iteration.
   bool disjoint() {
     std::vector<std::pair<Span*, Span*>> runs;
     for (const List& l : lists) {
