@@ -24,9 +24,9 @@ block's in 8.  skip_nonfinite leaves everything as it is in a step whose joint n
 
 A moment in 8 bits moves against its block's largest only once one step moves it by half a code's step.  So an element
 whose gradients stop while its block goes on keeps 0.5 % of the block's largest m (code 9 with beta1 = 0.9) and its share of
-the largest v (any code, with beta2 = 0.999), where in 32 bits both decay to zero: it goes on moving, a step
-by 5 % of lr if its gradients were a tenth of the largest, by 40 % if a hundredth, by nearly lr if less.  Parameters whose
-elements get gradients now and then (tables, rarely chosen rows) belong in 32 bits.
+the largest v (any code, with beta2 = 0.999), where in 32 bits both decay to zero: it goes on moving, a step by 5 % of lr if
+its gradients were a tenth of the largest, by 40 % if a hundredth, by nearly lr if less.  Parameters whose elements get
+gradients now and then (tables, rarely chosen rows) belong in 32 bits.
 
 Step counts live on the device (fp32, one per tensor), so that a step can be captured into a HIP graph and replayed; a
 learning rate that changes between replays is a one-element fp32 device tensor.  Calls enqueue work on the current stream
@@ -130,7 +130,8 @@ def _check_eps(eps, coded):
 
 
 def _check(params, grads, exp_avgs, exp_avg_sqs, scales, steps):
-    """Checks the lists of one device (steps: a tensor or a list of them); gradients that are laid out unlike their parameters come back as copies."""
+    """Checks the lists of one device (steps: a tensor or a list of them); gradients that are laid out unlike their
+    parameters come back as copies."""
     n = len(params)
     if not len(grads) == len(exp_avgs) == len(exp_avg_sqs) == n or (scales is not None and len(scales) != n):
         raise ValueError("params, grads and moments: lists of one length")
